@@ -224,6 +224,98 @@ typedef struct pa_qkv_prep_args {
 int pa_qkv_prep(const pa_qkv_prep_args* args, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Cross attention to an encoder's states, forward and backward: queries [batch, heads, seq_q,
+ * head_dim] against keys / values [kv_batch, kv_heads, seq_kv, head_dim] of another length.
+ * heads is a multiple of kv_heads (query head h reads key head h / (heads / kv_heads)); kv_batch is
+ * batch, or 1: one set of states for the whole batch. It is what the transformer blocks do with
+ * their text states (F.scaled_dot_product_attention with a short key sequence, routed by the modes
+ * of src/para_attn/para_attn_interface.py:279-495 or left to the framework by skip_small_kv), with
+ * what that call lacks here: shared key heads, masked keys that may hold anything, a form for
+ * single tokens, and gradients.
+ *
+ * Strides are element strides (batch, head, row); head_dim (64 or 128) is contiguous; base
+ * pointers and byte strides are multiples of 16 bytes. key_mask: one byte per key, non-zero = takes
+ * part, [batch][seq_kv] with a batch stride in bytes (0: one row for the whole batch), or NULL.
+ * Masked keys are never part of a sum, whatever they hold. A query without any key gives zeros, an
+ * LSE of -inf and no gradient; a key that no query sees has zero gradients.
+ *
+ * pa_xattn_fwd writes out and, if non-NULL, lse [batch, heads, seq_q] (fp32, natural log).
+ * pa_xattn_bwd reads q, k, v, out, lse (of the forward call) and dout and writes dq, dk, dv whole;
+ * with kv_batch = 1 dk and dv are the sums over the batch. Sums are fp32 in a fixed order: equal
+ * calls on equal devices give equal bits.
+ *
+ * workspace: pa_xattn_workspace_bytes(args, backward) bytes (0 possible; depends on the current
+ * device's SM count), 256-byte aligned; calls that may overlap must not share it. status and
+ * wait_limit_ns as in pa_attn_args. The device that owns the tensors must be current.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct pa_xattn_args {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;               /* read by the backward call */
+    float* lse;              /* read by the backward call */
+    const void* dout;        /* backward */
+    void* dq;
+    void* dk;
+    void* dv;
+    int32_t batch, kv_batch, heads, kv_heads, seq_q, seq_kv, head_dim;
+    int32_t dtype;           /* pa_dtype */
+    float scale;
+    int32_t pad_;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+    int64_t do_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+    const uint8_t* key_mask;
+    int64_t mask_stride;
+    int32_t* status;
+    uint64_t wait_limit_ns;
+    void* workspace;
+    int64_t workspace_bytes;
+} pa_xattn_args;
+
+int64_t pa_xattn_workspace_bytes(const pa_xattn_args* args, int32_t backward);
+int pa_xattn_fwd(const pa_xattn_args* args, void* stream);
+int pa_xattn_bwd(const pa_xattn_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Per-head RMSNorm of queries and keys with the position rotation in the same pass, and its
+ * gradients: y = R(row) (weight * x / sqrt(mean(x^2) + eps)) for every head vector x. The training
+ * counterpart of pa_qkv_prep's norm and rotation: one rounding at the end, separate head counts of
+ * q and k, both kinds of rotation pairs.
+ *
+ * x[0] (q), x[1] (k, may be NULL): [batch, rows, heads[i], head_dim], element strides (batch, row,
+ * head), head_dim (64 or 128) contiguous, base pointers and byte strides multiples of 16 bytes.
+ * weight[i]: [head_dim] in the tensors' dtype, 16-byte aligned, or NULL: no norm. cos / sin: fp32
+ * [>= table_row0 + rows, head_dim], 16-byte aligned, or both NULL: no rotation. Pairs are the adjacent
+ * elements (2i, 2i + 1) if interleaved, else (i, i + head_dim / 2): a' = a cos_a - c sin_a,
+ * c' = c cos_c + a sin_c.
+ *
+ * pa_qk_norm_fwd: y from x. pa_qk_norm_bwd: dx from x and dy and, where dweight[i] is non-NULL, the
+ * weights' gradients (workspace: pa_qk_norm_workspace_bytes() bytes, needed only then; calls that may
+ * overlap must not share it). Sums are fp32 in a fixed order.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct pa_qk_norm_args {
+    const void* x[2];
+    const void* dy[2];       /* backward */
+    void* y[2];              /* forward: outputs; backward: dx */
+    const void* weight[2];
+    void* dweight[2];        /* backward, each may be NULL */
+    int64_t x_stride[2][3], dy_stride[2][3], y_stride[2][3];
+    const float* cos;
+    const float* sin;
+    int64_t table_row0;
+    int32_t batch, rows, heads[2], head_dim;
+    int32_t dtype;           /* pa_dtype */
+    int32_t interleaved;
+    float eps;
+    void* workspace;
+    int64_t workspace_bytes;
+} pa_qk_norm_args;
+
+int64_t pa_qk_norm_workspace_bytes(void);
+int pa_qk_norm_fwd(const pa_qk_norm_args* args, void* stream);
+int pa_qk_norm_bwd(const pa_qk_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Exchange. Replaces the NCCL all_to_all_single calls of _sdpa_input_all_to_all /
  * _sdpa_output_all_to_all (src/para_attn/para_attn_interface.py:52-87, through
  * src/para_attn/primitives.py:72-78) and the K/V rotation of torch:_AllToAllRotater

@@ -102,6 +102,34 @@ class QkvPrepArgs(C.Structure):
     ]
 
 
+class XattnArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("dout", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("batch", C.c_int32), ("kv_batch", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+        ("seq_q", C.c_int32), ("seq_kv", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+        ("scale", C.c_float), ("pad_", C.c_int32),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("o_stride", C.c_int64 * 3), ("do_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3),
+        ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
+        ("key_mask", C.c_void_p), ("mask_stride", C.c_int64),
+        ("status", C.c_void_p), ("wait_limit_ns", C.c_uint64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class QkNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p * 2), ("dy", C.c_void_p * 2), ("y", C.c_void_p * 2),
+        ("weight", C.c_void_p * 2), ("dweight", C.c_void_p * 2),
+        ("x_stride", (C.c_int64 * 3) * 2), ("dy_stride", (C.c_int64 * 3) * 2), ("y_stride", (C.c_int64 * 3) * 2),
+        ("cos", C.c_void_p), ("sin", C.c_void_p), ("table_row0", C.c_int64),
+        ("batch", C.c_int32), ("rows", C.c_int32), ("heads", C.c_int32 * 2), ("head_dim", C.c_int32),
+        ("dtype", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
 _lib = None
 
 
@@ -128,6 +156,16 @@ def load() -> C.CDLL:
     lib.pa_attn_fwd.argtypes = [C.POINTER(AttnArgs), C.c_void_p]
     lib.pa_qkv_prep.restype = C.c_int
     lib.pa_qkv_prep.argtypes = [C.POINTER(QkvPrepArgs), C.c_void_p]
+    lib.pa_xattn_workspace_bytes.restype = C.c_int64
+    lib.pa_xattn_workspace_bytes.argtypes = [C.POINTER(XattnArgs), C.c_int32]
+    for fn in (lib.pa_xattn_fwd, lib.pa_xattn_bwd):
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(XattnArgs), C.c_void_p]
+    lib.pa_qk_norm_workspace_bytes.restype = C.c_int64
+    lib.pa_qk_norm_workspace_bytes.argtypes = []
+    for fn in (lib.pa_qk_norm_fwd, lib.pa_qk_norm_bwd):
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(QkNormArgs), C.c_void_p]
     lib.pa_cp_attn_fwd.restype = C.c_int
     lib.pa_cp_attn_fwd.argtypes = [C.POINTER(CpAttnArgs), C.c_void_p]
     lib.pa_taylor_update.restype = C.c_int

@@ -10,16 +10,17 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libpa_b200.so"
-SOURCES = ["pa_api.cu"]
+SOURCES = ["pa_api.cu", "pa_qk_norm.cu", "pa_xattn_fwd.cu", "pa_xattn_bwd.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -34,7 +35,7 @@ def _stale() -> bool:
     if not LIB_PATH.exists():
         return True
     built = LIB_PATH.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list((PKG_DIR.parent / "include").glob("*.h"))
+    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((PKG_DIR.parent / "include").glob("*.h"))
     return any(d.stat().st_mtime > built for d in deps)
 
 
@@ -45,12 +46,19 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     cmd = [_nvcc(), *NVCC_FLAGS]
     if verbose:
         cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", str(LIB_PATH), *[str(CSRC / s) for s in SOURCES], "-lcudart"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+    with tempfile.TemporaryDirectory() as tmp:
+        # one compiler per source, all at once: each takes most of a minute
+        objects = [str(Path(tmp) / (Path(src).stem + ".o")) for src in SOURCES]
+        running = [subprocess.Popen([*cmd, "-c", "-o", obj, str(CSRC / src)], stdout=subprocess.PIPE,
+                                    stderr=subprocess.STDOUT, text=True) for src, obj in zip(SOURCES, objects)]
+        logs = [p.communicate()[0] for p in running]
+        if any(p.returncode != 0 for p in running):
+            raise RuntimeError("nvcc failed:\n" + "".join(log for p, log in zip(running, logs) if p.returncode != 0))
+        res = subprocess.run([*cmd, "--shared", "-o", str(LIB_PATH), *objects, "-lcudart"], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
     if verbose:
-        sys.stderr.write(res.stderr)
+        sys.stderr.write("".join(logs))
     return LIB_PATH
 
 

@@ -14,12 +14,15 @@
 #include "fbc_sm100.cuh"
 #include "key_mask_sm100.cuh"
 #include "merge_sm100.cuh"
+#include "pa_host.h"
 #include "qkv_prep_sm100.cuh"
 #include "taylor_sm100.cuh"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}  // namespace
+
+namespace pa_host {
 
 int fail(int code, const char* fmt, ...) {
     va_list ap;
@@ -43,6 +46,7 @@ int sm_count() {
     return cached[dev];
 }
 
+namespace {
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -61,6 +65,8 @@ EncodeTiledFn get_encode_fn() {
     });
     return fn;
 }
+
+}  // namespace
 
 // 5-D map over [chunk][batch][head][row][head_dim] with element strides (head_dim stride 1); the box is
 // 64 elements x 128 rows with the 128-byte swizzle the MMA descriptors expect.
@@ -85,12 +91,28 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int head_dim, int ro
     cuuint32_t box[5] = {64, 128, 1, 1, 1};
     cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     CUtensorMapDataType dt = dtype == PA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUresult r = enc(map, dt, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return enc(map, dt, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // a thread that has not used the GPU yet (a backward pass runs on a thread of its own) has no
+        // context until a runtime call binds the device's
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+    }
     if (r != CUDA_SUCCESS) return fail(PA_ECUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", what, int(r));
     return PA_OK;
 }
+
+}  // namespace pa_host
+
+using pa_host::fail;
+using pa_host::make_map;
+using pa_host::sm_count;
+
+namespace {
 
 template <bool kBF16, bool kCausal, int kD, bool kSplit = false>
 int launch_attn_inst(const CUtensorMap* maps, const pa::AttnParams& p, const pa::PushParams& push, int grid,

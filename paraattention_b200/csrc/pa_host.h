@@ -1,0 +1,16 @@
+// Host helpers shared by the translation units behind the C ABI (defined in pa_api.cu).
+#pragma once
+#include <cuda.h>
+#include <cstdint>
+
+namespace pa_host {
+
+// Records a message for pa_last_error() and returns `code`.
+int fail(int code, const char* fmt, ...);
+// Streaming multiprocessors of the current device.
+int sm_count();
+// Tensor map over [chunk][batch][head][row][head_dim], element strides, 128-row boxes of 64 elements.
+int make_map(CUtensorMap* map, const void* base, int dtype, int head_dim, int rows, int heads, int batch, int chunks,
+             int64_t s_row, int64_t s_head, int64_t s_batch, int64_t s_chunk, const char* what);
+
+}  // namespace pa_host

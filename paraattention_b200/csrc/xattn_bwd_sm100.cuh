@@ -1,0 +1,573 @@
+// Cross attention backward for B200. With P = exp(s q k^T - lse), delta = rowsum(do * out):
+//   dP = do v^T,  dS = P * (dP - delta),  dq = s dS k,  dk = s dS^T q,  dv = P^T do.
+//
+// Two passes of ONE kernel: the query pass (kKeys = false) owns tiles of 128 query rows and walks
+// the key tiles for dq; the key pass (kKeys = true) owns tiles of 128 keys and walks the query
+// tiles (of every head that shares the key head, and of every batch entry that shares the keys)
+// for dk and dv. In both, the owned pair (X, Y) = (q, do) or (k, v) stays in shared memory, the
+// other pair (Z, W) = (k, v) or (q, do) streams through a two-stage ring, and per step
+//   T1 = X Z^T, T2 = Y W^T                (tensor core, into TMEM)
+//   P = 2^(T1 sl - lse'), dS = P (T2 - delta)   (one thread per owned row and half of the columns)
+//   A1 += dS Z  [, A2 += P W in the key pass]   (tensor core, dS and P as TMEM operands)
+// so dS and P never leave TMEM and are never transposed: the key pass computes their transposes
+// to begin with. The price is that S and dP are computed twice (7 products instead of 5); what it
+// buys is no atomics (sums in a fixed order), no fp32 dq traffic, and each gradient written once.
+//
+// As in the forward kernel a step is run as two halves of the streamed rows (columns of T), each
+// with its own chain T1, T2 -> elementwise -> A: warps 0-3 serve half 0, warps 4-7 half 1, and while one
+// half is in its elementwise phase the tensor core works on the other. TMEM columns: T1 [0,128),
+// T2 [128,256), A1 [256, 256 + D), A2 [256 + D, 256 + 2 D); dS overwrites T2, P overwrites T1.
+// CTAs are persistent and the roles run ahead across units (xattn_sm100.cuh divides the work).
+//
+// What is rounded: P and dS to the tensors' 16-bit type, as operands of a 16-bit product (their
+// relative error, half an ulp, averages out over the sum); everything else is fp32.
+#pragma once
+#include "fbc_sm100.cuh"
+#include "xattn_sm100.cuh"
+
+namespace pa {
+
+struct XBwdParams {
+    int batch, kv_batch, hkv, group, sq, skv;
+    int mt, kt;       // 128-row tiles of the queries / of the keys
+    float scale, scale_log2;
+    uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv
+    long long g_sb[2], g_sh[2], g_ss[2];
+    // [B][Hq][mt * 128] (lse * log2 e, delta); rows behind the last query, and rows without any key, have
+    // (+inf, 0), which makes their P zero
+    const float2* stats;
+    const unsigned long long* words;
+    const int* extent;
+    XSched sched;
+    float* part;      // [slot][A1, A2][D / 4][128 rows][4]
+    int* status;
+    unsigned long long wait_ns;
+};
+
+struct XBwdCtl {
+    uint64_t xy_full, xy_empty;
+    uint64_t zw_full[2], zw_empty[2], z_clean[2];
+    uint64_t t_full[2];   // T1 and T2 of a half are in TMEM
+    uint64_t p_full[2];   // dS and P of a half are in TMEM (128 arrivals)
+    uint64_t acc_done;    // A1, A2 of a segment are complete
+    uint64_t acc_free;    // the epilogue has read them (256 arrivals)
+    uint64_t teardown;
+    uint32_t tmem_base;
+    int abort;
+};
+constexpr int kXBwdStatBytes = 2 * kTileN * 8;
+constexpr int kXBwdSmemBytes = 1024 + 6 * kTileBytes + kXBwdStatBytes + 512;
+static_assert(sizeof(XBwdCtl) <= 512, "control block too large");
+static_assert(kXBwdSmemBytes <= 232448, "shared memory");
+
+// Where a segment's owned tile and a step's streamed tile lie.
+struct XBwdUnit {
+    int b, head, tile;  // owned tile: batch entry (of its tensor), head (of its tensor), 128-row tile
+    int t0, t1;
+};
+struct XBwdStep {
+    int b, head, tile;  // streamed tile
+};
+
+template <bool kKeys>
+__device__ __forceinline__ XBwdUnit x_bwd_unit(const XBwdParams& p, const XSeg& g) {
+    XBwdUnit u;
+    int x = g.unit;
+    const int tiles = kKeys ? p.kt : p.mt, heads = kKeys ? p.hkv : p.hkv * p.group;
+    u.tile = x % tiles;
+    x /= tiles;
+    u.head = x % heads;
+    u.b = x / heads;
+    u.t0 = g.t0;
+    u.t1 = g.t1;
+    if (!kKeys && p.extent != nullptr) {  // key tiles behind the last key that takes part
+        const int n = (__ldg(p.extent + u.b) + kTileN - 1) / kTileN;
+        u.t1 = min(u.t1, n);
+        u.t0 = min(u.t0, u.t1);
+    }
+    return u;
+}
+// Key pass: steps run over (batch entries that share the keys, heads of the group, query tiles).
+template <bool kKeys>
+__device__ __forceinline__ XBwdStep x_bwd_step(const XBwdParams& p, const XBwdUnit& u, int step) {
+    XBwdStep s;
+    if (!kKeys) {
+        s.b = p.kv_batch == 1 ? 0 : u.b;
+        s.head = u.head / p.group;
+        s.tile = step;
+        return s;
+    }
+    const int m = step / p.mt;
+    s.tile = step - m * p.mt;
+    const int bb = m / p.group;
+    s.head = u.head * p.group + (m - bb * p.group);
+    s.b = p.kv_batch == 1 ? bb : u.b;
+    return s;
+}
+// The first step >= `step` with something to do (the segment's end if none): the key pass skips batch
+// entries whose mask ends before the owned keys.
+template <bool kKeys>
+__device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u, int step) {
+    if (!kKeys || p.extent == nullptr) return step;
+    const int per_b = p.group * p.mt;
+    while (step < u.t1) {
+        const int b = p.kv_batch == 1 ? step / per_b : u.b;
+        if (u.tile * kTileN < __ldg(p.extent + b)) return step;
+        if (p.kv_batch != 1) return u.t1;
+        step = (b + 1) * per_b;
+    }
+    return u.t1;
+}
+
+template <bool kBF16, int kD, bool kKeys>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y,
+                 const __grid_constant__ CUtensorMap tm_z, const __grid_constant__ CUtensorMap tm_w,
+                 const __grid_constant__ XBwdParams p) {
+    constexpr int kAtoms = kD / 64;
+    constexpr int kOperandBytes = kAtoms * kHalfBytes;
+    constexpr uint32_t kColT1 = 0, kColT2 = 128, kColA1 = 256, kColA2 = 256 + kD;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+    const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sX + 4 * kTileBytes;
+    float2* stat = reinterpret_cast<float2*>(smem + 6 * kTileBytes);  // [stage][128], key pass
+    XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + 6 * kTileBytes + kXBwdStatBytes);
+    volatile int* s_abort = &ctl->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) ctl->abort = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+    __syncthreads();
+    if (ctl->abort != 0) return;
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&ctl->xy_full), 1);
+        mbar_init(smem_u32(&ctl->xy_empty), 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_u32(&ctl->zw_full[s]), 1);
+            mbar_init(smem_u32(&ctl->zw_empty[s]), 1);
+            mbar_init(smem_u32(&ctl->z_clean[s]), 1);
+            mbar_init(smem_u32(&ctl->t_full[s]), 1);
+            mbar_init(smem_u32(&ctl->p_full[s]), 128);
+        }
+        mbar_init(smem_u32(&ctl->acc_done), 1);
+        mbar_init(smem_u32(&ctl->acc_free), 256);
+        mbar_init(smem_u32(&ctl->teardown), 1);
+        mbar_init_fence();
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
+        tmem_relinquish();
+    }
+    if (warp == kTmaWarp && lane == 0) {
+        tma_prefetch_desc(&tm_x);
+        tma_prefetch_desc(&tm_y);
+        tma_prefetch_desc(&tm_z);
+        tma_prefetch_desc(&tm_w);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
+    const uint64_t limit = p.wait_ns;
+    const int n_words = (p.skv + 63) >> 6;
+    const bool clean = !kKeys && p.words != nullptr;  // masked rows of K are zeroed before use
+
+    XCursor cursor(p.sched);
+    XSeg seg;
+    if (warp == kTmaWarp) {
+        // =============================== TMA producer ======================================
+        if (lane == 0) {
+            bool ok = true;
+            int j = 0, n_seg = 0;
+            while (ok && cursor.next(p.sched, seg)) {
+                const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
+                int st = x_bwd_live<kKeys>(p, u, u.t0);
+                if (st >= u.t1) continue;
+                if (n_seg > 0) ok = mbar_wait(smem_u32(&ctl->xy_empty), (n_seg - 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                if (!ok) break;
+                const uint32_t bx = smem_u32(&ctl->xy_full);
+                mbar_expect_tx(bx, 2 * kOperandBytes);
+#pragma unroll
+                for (int h = 0; h < kAtoms; ++h) {
+                    tma_load_5d(sX + h * kHalfBytes, &tm_x, bx, h * 64, u.tile * kTileM, u.head, u.b, 0);
+                    tma_load_5d(sY + h * kHalfBytes, &tm_y, bx, h * 64, u.tile * kTileM, u.head, u.b, 0);
+                }
+                for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
+                    const XBwdStep s = x_bwd_step<kKeys>(p, u, st);
+                    const int sg = j & 1;
+                    const uint32_t bz = smem_u32(&ctl->zw_full[sg]);
+                    if (j >= 2) ok = mbar_wait(smem_u32(&ctl->zw_empty[sg]), ((j >> 1) & 1) ^ 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                    if (!ok) break;
+                    mbar_expect_tx(bz, 2 * kOperandBytes + (kKeys ? kTileN * 8 : 0));
+#pragma unroll
+                    for (int h = 0; h < kAtoms; ++h) {
+                        tma_load_5d(sZ + sg * kTileBytes + h * kHalfBytes, &tm_z, bz, h * 64, s.tile * kTileN, s.head, s.b, 0);
+                        tma_load_5d(sW + sg * kTileBytes + h * kHalfBytes, &tm_w, bz, h * 64, s.tile * kTileN, s.head, s.b, 0);
+                    }
+                    if (kKeys) {
+                        const float2* src = p.stats + ((static_cast<long long>(s.b) * p.hkv * p.group + s.head) * p.mt + s.tile) * kTileN;
+                        asm volatile(
+                            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                smem_u32(stat + sg * kTileN)),
+                            "l"(src), "r"(kTileN * 8), "r"(bz)
+                            : "memory");
+                    }
+                }
+                ++n_seg;
+            }
+            if (*s_abort != 0) {  // leave only once copies already issued have landed (bounded)
+                int none = 0;
+                volatile int* no_abort = &none;
+                if (n_seg > 0) mbar_wait(smem_u32(&ctl->xy_full), (n_seg - 1) & 1, no_abort, nullptr, 10000000ull, 0);
+                mbar_wait(smem_u32(&ctl->xy_full), n_seg & 1, no_abort, nullptr, 10000000ull, 0);
+                for (int jj = (j > 2 ? j - 2 : 0); jj <= j; ++jj)
+                    mbar_wait(smem_u32(&ctl->zw_full[jj & 1]), (jj >> 1) & 1, no_abort, nullptr, 10000000ull, 0);
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        // =============================== MMA issuer ========================================
+        constexpr uint32_t idesc_t = make_idesc_f16(kBF16, false, kTileM, 64);
+        constexpr uint32_t idesc_a = make_idesc_f16(kBF16, true, kTileM, kD);
+        const uint32_t leader = elect_one() ? 1u : 0u;
+        // K-major descriptors (T1, T2) and MN-major descriptors (the same tiles as B operands of A1, A2)
+        const uint64_t dk0 = smem_desc_sw128(sX, 16, 1024), dm0 = smem_desc_sw128(sZ, kHalfBytes, 1024);
+        const uint32_t hi_k = static_cast<uint32_t>(dk0 >> 32), hi_m = static_cast<uint32_t>(dm0 >> 32);
+        const uint32_t lo_x = static_cast<uint32_t>(dk0), lo_y = lo_x + (kTileBytes >> 4);
+        const uint32_t lo_z = static_cast<uint32_t>(smem_desc_sw128(sZ, 16, 1024)), lo_w = lo_z + (2 * kTileBytes >> 4);
+        const uint32_t lo_zm = static_cast<uint32_t>(dm0), lo_wm = lo_zm + (2 * kTileBytes >> 4);
+        auto issue_t = [&](int sg, int half) {
+            const uint32_t zo = (sg * kTileBytes + half * 64 * 128) >> 4;
+#pragma unroll
+            for (int ks = 0; ks < kD / 16; ++ks) {
+                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                tc_mma_ss_elect(tmem + kColT1 + half * 64, lo_x + off, hi_k, lo_z + zo + off, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+            }
+#pragma unroll
+            for (int ks = 0; ks < kD / 16; ++ks) {
+                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                tc_mma_ss_elect(tmem + kColT2 + half * 64, lo_y + off, hi_k, lo_w + zo + off, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+            }
+            tc_commit_elect(smem_u32(&ctl->t_full[half]), leader);
+        };
+        auto issue_a = [&](int sg, int half, bool acc) {
+            const uint32_t so = (sg * kTileBytes + half * 64 * 128) >> 4;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+                tc_mma_ts_elect(tmem + kColA1, tmem + kColT2 + half * 64 + ks * 8, lo_zm + so + ((ks * 16 * 128) >> 4), hi_m,
+                                idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
+            if (kKeys) {
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    tc_mma_ts_elect(tmem + kColA2, tmem + kColT1 + half * 64 + ks * 8, lo_wm + so + ((ks * 16 * 128) >> 4), hi_m,
+                                    idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
+            }
+        };
+        auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+            const bool r = mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+            return __all_sync(0xffffffffu, r);
+        };
+        auto wait_zw = [&](int j) -> bool {
+            return wait(clean ? &ctl->z_clean[j & 1] : &ctl->zw_full[j & 1], (j >> 1) & 1);
+        };
+        bool ok = true, issued = false;
+        int j = 0, n_seg = 0;  // steps, segments with steps
+        while (ok && cursor.next(p.sched, seg)) {
+            const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
+            int st = x_bwd_live<kKeys>(p, u, u.t0);
+            if (st >= u.t1) continue;
+            int nx = x_bwd_live<kKeys>(p, u, st + 1);
+            ok = wait(&ctl->xy_full, n_seg & 1) && wait_zw(j);
+            if (!ok) break;
+            tc_fence_after();
+            issued = true;
+            issue_t(j & 1, 0);
+            issue_t(j & 1, 1);
+            if (nx >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
+            bool first = true;
+            while (true) {
+                const bool more = nx < u.t1;
+                int nx2 = nx;
+                if (more) {
+                    nx2 = x_bwd_live<kKeys>(p, u, nx + 1);
+                    ok = wait_zw(j + 1);
+                    if (!ok) break;
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    ok = wait(&ctl->p_full[half], j & 1);
+                    // (the accumulators of the segment before have been read by the epilogue)
+                    if (ok && first && half == 0 && n_seg > 0) ok = wait(&ctl->acc_free, (n_seg - 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_a(j & 1, half, !first || half > 0);
+                    if (half == 1) tc_commit_elect(smem_u32(&ctl->zw_empty[j & 1]), leader);
+                    if (more) issue_t((j + 1) & 1, half);
+                }
+                if (!ok) break;
+                if (more && nx2 >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
+                ++j;
+                first = false;
+                if (!more) break;
+                st = nx;
+                nx = nx2;
+            }
+            if (!ok) break;
+            tc_commit_elect(smem_u32(&ctl->acc_done), leader);
+            ++n_seg;
+        }
+        if (!ok && issued) {
+            int none = 0;
+            volatile int* no_abort = &none;
+            tc_commit_elect(smem_u32(&ctl->teardown), leader);
+            mbar_wait(smem_u32(&ctl->teardown), 0, no_abort, nullptr, 100000000ull, 0);
+        }
+    } else if (warp == kTmaWarp + 1 && clean) {
+        // =============================== masked rows of K ==================================
+        bool ok = true;
+        int j = 0;
+        while (ok && cursor.next(p.sched, seg)) {
+            const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
+            const unsigned long long* row = p.words + static_cast<long long>(u.b) * n_words;
+            for (int t = u.t0; t < u.t1; ++t, ++j) {
+                const int sg = j & 1;
+                const unsigned long long w0 = x_key_word(row, p.skv, t, 0), w1 = x_key_word(row, p.skv, t, 1);
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->zw_full[sg]), (j >> 1) & 1, s_abort, p.status, limit,
+                                                       PA_DEV_TIMEOUT_PIPE));
+                if (!ok) break;
+                if ((w0 & w1) != ~0ull) {
+                    x_zero_rows<kD>(smem + 2 * kTileBytes + sg * kTileBytes, w0, w1, lane);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->z_clean[sg]));
+            }
+        }
+    } else if (warp < kSoftmaxWarps) {
+        // =============================== elementwise + epilogue ============================
+        const int quarter = warp & 3, half = warp >> 2;
+        const int row_in_tile = quarter * 32 + lane;
+        const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t t1 = tmem + lane_base + kColT1 + half * 64, t2 = tmem + lane_base + kColT2 + half * 64;
+        const float sl = p.scale_log2;
+        const float2 sl2 = make_float2(sl, sl);
+        bool ok = true;
+        int j = 0, n_seg = 0;
+        while (ok && cursor.next(p.sched, seg)) {
+            const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
+            int st = x_bwd_live<kKeys>(p, u, u.t0);
+            const bool any = st < u.t1;
+            const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
+            float2 mine = make_float2(0.f, 0.f);
+            if (!kKeys)
+                mine = __ldg(p.stats + (static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt * kTileM + row);
+            for (; st < u.t1 && ok; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
+                unsigned long long word = ~0ull;  // query pass: my half's keys; key pass: all or nothing
+                if (!kKeys) {
+                    word = x_key_word(p.words != nullptr ? p.words + static_cast<long long>(u.b) * n_words : nullptr, p.skv, st, half);
+                } else if (p.words != nullptr) {
+                    const int b = x_bwd_step<kKeys>(p, u, st).b;
+                    if (row >= p.skv || ((__ldg(p.words + static_cast<long long>(b) * n_words + (row >> 6)) >> (row & 63)) & 1ull) == 0) word = 0ull;
+                } else if (row >= p.skv) {
+                    word = 0ull;
+                }
+                const bool plain = __all_sync(0xffffffffu, word == ~0ull);
+                if (kKeys)  // (the step's statistics are in shared memory: already true when t_full is)
+                    ok = mbar_wait(smem_u32(&ctl->zw_full[j & 1]), (j >> 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                ok = mbar_wait(smem_u32(&ctl->t_full[half]), j & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE) && ok;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const float4* col = reinterpret_cast<const float4*>(stat + (j & 1) * kTileN + half * 64);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t a[32], d[32], pp[16], ds[16];
+                    tmem_ld32(t1 + c * 32, a);
+                    tmem_ld32(t2 + c * 32, d);
+                    tc_wait_ld();
+                    tmem_ld_fence(a);
+                    tmem_ld_fence(d);
+                    const uint32_t live = static_cast<uint32_t>(word >> (c * 32));
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float2 neg, dl;
+                        if (kKeys) {
+                            const float4 s4 = col[c * 16 + (i >> 1)];
+                            neg = make_float2(-s4.x, -s4.z);
+                            dl = make_float2(-s4.y, -s4.w);
+                        } else {
+                            neg = make_float2(-mine.x, -mine.x);
+                            dl = make_float2(-mine.y, -mine.y);
+                        }
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), sl2, neg);
+                        float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                        const float2 t = __fadd2_rn(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), dl);
+                        float2 s = __fmul2_rn(e, t);
+                        if (!plain) {
+                            if (((live >> i) & 1u) == 0) e.x = s.x = 0.f;
+                            if (((live >> (i + 1)) & 1u) == 0) e.y = s.y = 0.f;
+                        }
+                        if (kKeys) pp[i >> 1] = kBF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+                        ds[i >> 1] = kBF16 ? pack_bf16x2(s.x, s.y) : pack_f16x2(s.x, s.y);
+                    }
+                    tmem_st16(t2 + c * 16, ds);
+                    if (kKeys) tmem_st16(t1 + c * 16, pp);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(smem_u32(&ctl->p_full[half]));
+            }
+            if (any && ok) {
+                ok = mbar_wait(smem_u32(&ctl->acc_done), n_seg & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                ++n_seg;
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            // Key pass: warps 0-3 write dk, warps 4-7 dv. Query pass: each half of the warps writes half
+            // of dq's columns.
+            const int which = kKeys ? half : 0;
+            constexpr int kBlocks = kKeys ? kD / 32 : kD / 64;
+            const int block0 = kKeys ? 0 : half * kBlocks;
+            const uint32_t ta = tmem + lane_base + (which ? kColA2 : kColA1);
+            const float factor = which ? 1.0f : p.scale;
+            const bool in_range = row < (kKeys ? p.skv : p.sq);
+            uint16_t* grow = p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]);
+            float4* part = reinterpret_cast<float4*>(p.part) +
+                           (static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) * kTileM + row_in_tile;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const int blk = block0 + b;
+                uint32_t o[32];
+                tmem_ld32(ta + blk * 32, o);
+                tc_wait_ld();
+                tmem_ld_fence(o);
+                if (!any) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+                }
+                if (seg.slot >= 0) {
+#pragma unroll
+                    for (int v4 = 0; v4 < 8; ++v4)
+                        __stcg(part + (blk * 8 + v4) * kTileM,
+                               make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
+                                           __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
+                } else if (in_range) {
+#pragma unroll
+                    for (int v4 = 0; v4 < 4; ++v4) {
+                        uint32_t q[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float f0 = __uint_as_float(o[v4 * 8 + 2 * x]) * factor;
+                            const float f1 = __uint_as_float(o[v4 * 8 + 2 * x + 1]) * factor;
+                            q[x] = kBF16 ? pack_bf16x2(f0, f1) : pack_f16x2(f0, f1);
+                        }
+                        *reinterpret_cast<uint4*>(grow + blk * 32 + v4 * 8) = make_uint4(q[0], q[1], q[2], q[3]);
+                    }
+                }
+            }
+            if (any) {
+                tc_fence_before();
+                mbar_arrive(smem_u32(&ctl->acc_free));
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Adds the partial results of units that several CTAs worked on, in range order: one block per
+// unit, 32 columns and accumulator, one thread per row.
+template <bool kBF16, int kD, bool kKeys>
+__global__ void __launch_bounds__(128)
+xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, int grid) {
+    const int unit = blockIdx.x, cols0 = blockIdx.y * 32, which = blockIdx.z, r = threadIdx.x;
+    float acc[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    if (!x_for_parts(p.sched, unit, grid, [&](int, int slot) {
+            const float4* src = reinterpret_cast<const float4*>(p.part) +
+                                ((static_cast<long long>(slot) * 2 + which) * (kD / 4) + cols0 / 4) * kTileM + r;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+                const float4 x = __ldcg(src + v * kTileM);
+                acc[4 * v] += x.x;
+                acc[4 * v + 1] += x.y;
+                acc[4 * v + 2] += x.z;
+                acc[4 * v + 3] += x.w;
+            }
+        }))
+        return;
+    XSeg g;
+    g.unit = unit;
+    g.t0 = g.t1 = 0;
+    const XBwdUnit u = x_bwd_unit<kKeys>(p, g);
+    const int row = u.tile * kTileM + r;
+    if (row >= (kKeys ? p.skv : p.sq)) return;
+    const float factor = which ? 1.0f : p.scale;
+    uint16_t* grow = p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]) + cols0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        uint32_t q[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            q[x] = kBF16 ? pack_bf16x2(acc[v * 8 + 2 * x] * factor, acc[v * 8 + 2 * x + 1] * factor)
+                         : pack_f16x2(acc[v * 8 + 2 * x] * factor, acc[v * 8 + 2 * x + 1] * factor);
+        *reinterpret_cast<uint4*>(grow + v * 8) = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+}
+
+// stats[b][h][row] = (lse * log2 e, sum_d do * out) for the query rows, (+inf, 0) for rows without
+// any key and behind the last one. HBM-bound: one pass over do and out, 16 bytes per lane.
+struct XStatParams {
+    const uint16_t *o, *g;  // out, do
+    long long o_s[3], g_s[3];
+    const float* lse;  // [B][Hq][Sq]
+    float2* stats;     // [B][Hq][padded]
+    int batch, heads, sq, padded;
+};
+constexpr int kXStatThreads = 256;
+template <bool kBF16, int kD>
+__global__ void __launch_bounds__(kXStatThreads)
+xattn_stat_kernel(const __grid_constant__ XStatParams p) {
+    constexpr int kLanes = kD / 8;
+    const int at = (threadIdx.x % kLanes) * 8;
+    const unsigned n = static_cast<unsigned>(p.batch) * p.heads * p.padded;  // (the host has checked the range)
+    const unsigned step = gridDim.x * (kXStatThreads / kLanes);
+    // (heads innermost: neighbouring lanes read neighbouring heads of [B, S, H, D] memory. The trip count
+    // is the same for all lanes of a warp - the shuffles need them all.)
+    for (unsigned base = blockIdx.x * (kXStatThreads / kLanes); base < n; base += step) {
+        const unsigned idx = base + threadIdx.x / kLanes;
+        const unsigned t = idx / static_cast<unsigned>(p.heads);
+        const int h = static_cast<int>(idx - t * p.heads);
+        const int b = static_cast<int>(t / static_cast<unsigned>(p.padded));
+        const int s = static_cast<int>(t) - b * p.padded;
+        const bool live = idx < n && s < p.sq;
+        float dot = 0.f;
+        if (live) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.o + (b * p.o_s[0] + h * p.o_s[1] + s * p.o_s[2]) + at));
+            const uint4 y = __ldg(reinterpret_cast<const uint4*>(p.g + (b * p.g_s[0] + h * p.g_s[1] + s * p.g_s[2]) + at));
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dot = fmaf(lo16<kBF16>(xs[i]), lo16<kBF16>(ys[i]), dot);
+                dot = fmaf(hi16<kBF16>(xs[i]), hi16<kBF16>(ys[i]), dot);
+            }
+        }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (at == 0 && idx < n) {
+            float2 r = make_float2(INFINITY, 0.f);
+            if (live) {
+                const float l = __ldg(p.lse + (static_cast<long long>(b) * p.heads + h) * p.sq + s);
+                if (l != -INFINITY) r = make_float2(l * 1.4426950408889634f, dot);
+            }
+            p.stats[(static_cast<long long>(b) * p.heads + h) * p.padded + s] = r;
+        }
+    }
+}
+
+}  // namespace pa

@@ -1,0 +1,144 @@
+// Cross attention to an encoder's states: what the forward and the backward kernel share - how
+// the work is divided over persistent CTAs, and the key mask.
+//
+// Queries [B, Hq, Sq, D] attend to keys / values [B or 1, Hkv, Skv, D] of another length; `group`
+// = Hq / Hkv query heads share a key / value head; a boolean mask [B, Skv] drops keys.
+#pragma once
+#include <cstdint>
+
+#include "attn_common_sm100.cuh"
+
+namespace pa {
+
+// ---- division of the work -----------------------------------------------------------------
+// A kernel has `units` output tiles, each of which walks `steps` tiles of the other operand. The
+// grid is one CTA per SM. Whole units (split = 0): unit u belongs to CTA u % grid, so CTAs that
+// run at the same time share a head's operands in L2. Split (few units, or a poorly filled last
+// round): the list of all units * steps steps is cut into equal contiguous ranges, one per CTA; a
+// unit cut by a range boundary leaves fp32 partial results in a workspace slot of each CTA that
+// has a part of it, and a second launch adds them in range order (results do not depend on
+// scheduling). A CTA has at most one segment that begins inside a unit (slot 2 * CTA) and one
+// that begins with its unit but ends inside it (slot 2 * CTA + 1).
+struct XSched {
+    int units, steps, split;
+    long long total;  // units * steps
+};
+
+struct XSeg {
+    int unit, t0, t1;
+    int slot;  // -1: the whole unit is mine
+};
+
+__host__ __device__ inline long long x_range_begin(const XSched& s, int cta, int grid) {
+    return s.total * cta / grid;
+}
+// The CTA whose range holds step `pos`.
+__host__ __device__ inline int x_cta_of(const XSched& s, long long pos, int grid) {
+    int c = static_cast<int>(pos * grid / s.total);
+    while (c > 0 && x_range_begin(s, c, grid) > pos) --c;
+    while (c + 1 < grid && x_range_begin(s, c + 1, grid) <= pos) ++c;
+    return c;
+}
+
+struct XCursor {
+    long long pos, end;
+    __device__ __forceinline__ explicit XCursor(const XSched& s) {
+        if (s.split) {
+            pos = x_range_begin(s, blockIdx.x, gridDim.x);
+            end = x_range_begin(s, blockIdx.x + 1, gridDim.x);
+        } else {
+            pos = blockIdx.x;
+            end = s.units;
+        }
+    }
+    __device__ __forceinline__ bool next(const XSched& s, XSeg& g) {
+        if (pos >= end) return false;
+        if (!s.split) {
+            g.unit = static_cast<int>(pos);
+            g.t0 = 0;
+            g.t1 = s.steps;
+            g.slot = -1;
+            pos += gridDim.x;
+            return true;
+        }
+        g.unit = static_cast<int>(pos / s.steps);
+        g.t0 = static_cast<int>(pos - static_cast<long long>(g.unit) * s.steps);
+        const long long left = end - pos;
+        g.t1 = left < s.steps - g.t0 ? g.t0 + static_cast<int>(left) : s.steps;
+        g.slot = (g.t0 == 0 && g.t1 == s.steps) ? -1 : 2 * static_cast<int>(blockIdx.x) + (g.t0 > 0 ? 0 : 1);
+        pos += g.t1 - g.t0;
+        return true;
+    }
+};
+
+// Calls f(cta, slot) for the CTAs that hold a part of `unit`, in range order; false if one CTA
+// has all of it (then the result is already final).
+template <typename F>
+__device__ __forceinline__ bool x_for_parts(const XSched& s, int unit, int grid, F f) {
+    const long long a = static_cast<long long>(unit) * s.steps, b = a + s.steps;
+    int c = x_cta_of(s, a, grid);
+    if (x_range_begin(s, c + 1, grid) >= b) return false;
+    for (; c < grid; ++c) {
+        const long long r0 = x_range_begin(s, c, grid);
+        if (r0 >= b) break;
+        if (x_range_begin(s, c + 1, grid) == r0) continue;  // (an empty range)
+        f(c, 2 * c + (r0 > a ? 0 : 1));
+    }
+    return true;
+}
+
+// ---- key mask -------------------------------------------------------------------------------
+// mask [B][Skv] bytes -> words[b][Skv / 64 rounded up], bit i of word w = key 64 w + i, and
+// extent[b] = 1 + last key that takes part (0: none), by which the kernels skip what lies behind.
+constexpr int kXMaskThreads = 256;
+static __global__ void __launch_bounds__(kXMaskThreads)
+xattn_mask_kernel(const uint8_t* __restrict__ mask, long long batch_stride, int keys,
+                  unsigned long long* __restrict__ words, int* __restrict__ extent) {
+    __shared__ int last[kXMaskThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (keys + 63) / 64;
+    const uint8_t* src = mask + blockIdx.x * batch_stride;
+    unsigned long long* dst = words + static_cast<long long>(blockIdx.x) * n;
+    int mine = 0;
+    for (int w = warp; w < n; w += kXMaskThreads / 32) {
+        const int k = w * 64 + lane;
+        const unsigned lo = __ballot_sync(0xffffffffu, k < keys && src[k] != 0);
+        const unsigned hi = __ballot_sync(0xffffffffu, k + 32 < keys && src[k + 32] != 0);
+        if (lane == 0) dst[w] = lo | (static_cast<unsigned long long>(hi) << 32);
+        if (hi != 0) mine = w * 64 + 64 - __clz(hi);
+        else if (lo != 0) mine = w * 64 + 32 - __clz(lo);
+    }
+    if (lane == 0) last[warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < kXMaskThreads / 32; ++i) mine = max(mine, last[i]);
+        extent[blockIdx.x] = mine;
+    }
+}
+
+// A key tile's word for columns [64 half, 64 half + 64): keys that exist and that the mask keeps.
+__device__ __forceinline__ unsigned long long x_key_word(const unsigned long long* words, int keys, int tile, int half) {
+    const int k0 = tile * kTileN + half * 64;
+    if (k0 >= keys) return 0ull;
+    if (words != nullptr) return __ldg(words + (k0 >> 6));
+    const int n = keys - k0;
+    return n >= 64 ? ~0ull : (1ull << n) - 1ull;
+}
+
+// Zeroes the rows of a loaded key / value tile (two 64-row words, clear bit = row is masked) in
+// shared memory. The products with masked rows are multiplied by zero weights; this keeps
+// infinities and NaN that such rows may hold out of the sums. One whole warp calls.
+template <int kD>
+__device__ __forceinline__ void x_zero_rows(uint8_t* tile, unsigned long long w0, unsigned long long w1, int lane) {
+    constexpr int kChunks = kD / 8;  // 16-byte chunks per row
+    constexpr int kRows = 32 / kChunks;
+    const int chunk = lane % kChunks, sub = lane / kChunks;
+    uint8_t* base = tile + (chunk / 8) * kHalfBytes + (chunk % 8) * 16;
+    for (int r0 = 0; r0 < kTileN; r0 += kRows) {
+        const int r = r0 + sub;
+        const unsigned long long w = r < 64 ? w0 : w1;
+        if (((w >> (r & 63)) & 1ull) == 0) *reinterpret_cast<uint4*>(base + r * 128) = make_uint4(0, 0, 0, 0);
+    }
+}
+
+}  // namespace pa

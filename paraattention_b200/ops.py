@@ -29,6 +29,8 @@ __all__ = [
     "merge_out_lse_",
     "raw_attention_forward",
     "qkv_prepare",
+    "cross_attention",
+    "qk_norm_rotary",
 ]
 
 _DTYPES = {torch.bfloat16: L.PA_BF16, torch.float16: L.PA_F16}
@@ -349,3 +351,6 @@ def merge_out_lse_(acc_out: torch.Tensor, acc_lse: torch.Tensor, block_out: torc
     L.check(L.load().pa_merge_out_lse(acc_out.data_ptr(), acc_lse.data_ptr(), block_out.data_ptr(), block_lse.data_ptr(),
                                       acc_lse.numel(), acc_out.shape[-1], code,
                                       torch.cuda.current_stream(acc_out.device).cuda_stream))
+
+
+from .block_ops import cross_attention, qk_norm_rotary  # noqa: E402
