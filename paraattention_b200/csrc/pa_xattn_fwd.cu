@@ -84,10 +84,11 @@ int run_few(const pa_xattn_args* a, cudaStream_t s) {
 
 template <bool kBF16, int kD>
 int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo;
     int rc = make_map(&mq, a->q, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->q_stride[2], a->q_stride[1], a->q_stride[0], 0, "q");
     if (rc == PA_OK) rc = make_map(&mk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k");
     if (rc == PA_OK) rc = make_map(&mv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v");
+    if (rc == PA_OK) rc = make_map(&mo, a->out, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->o_stride[2], a->o_stride[1], a->o_stride[0], 0, "out", 32);
     if (rc != PA_OK) return rc;
     pa::XFwdParams p;
     memset(&p, 0, sizeof(p));
@@ -125,7 +126,7 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     auto kern = pa::xattn_fwd_kernel<kBF16, kD>;
     rc = allow_smem(kern, pa::kXFwdSmemBytes, "xattn forward");
     if (rc != PA_OK) return rc;
-    kern<<<f.grid, pa::kAttnThreads, pa::kXFwdSmemBytes, s>>>(mq, mk, mv, p);
+    kern<<<f.grid, pa::kAttnThreads, pa::kXFwdSmemBytes, s>>>(mq, mk, mv, mo, p);
     rc = launched("xattn forward");
     if (rc != PA_OK || !f.sched.split) return rc;
     pa::xattn_fwd_join_kernel<kBF16, kD><<<dim3(f.sched.units, kD / 32), 256, 0, s>>>(p, f.grid);

@@ -25,9 +25,9 @@ namespace pa {
 struct XFwdParams {
     int batch, kv_batch, hkv, group, sq, skv, mt;
     float scale, scale_log2;
-    uint16_t* out;
-    float* lse;  // [B][Hq][Sq] or NULL
+    uint16_t* out;  // (the joining kernel's; the main kernel stores through its tensor map)
     long long o_sb, o_sh, o_ss;
+    float* lse;  // [B][Hq][Sq] or NULL
     const unsigned long long* words;  // key mask, or NULL
     const int* extent;
     XSched sched;
@@ -47,7 +47,9 @@ struct XFwdCtl {
     uint32_t tmem_base;
     int abort;
 };
-constexpr int kXFwdSmemBytes = 1024 + 6 * kTileBytes + 512;  // alignment slack; Q, K and V ring; control block
+// alignment slack; Q, K and V ring; output staging of the 8 softmax warps; control block
+constexpr int kXFwdSmemBytes = 1024 + 6 * kTileBytes + kSoftmaxWarps * kXStageBytes + 512;
+static_assert(kXFwdSmemBytes <= 232448, "shared memory");
 static_assert(sizeof(XFwdCtl) <= 512, "control block too large");
 
 // What a segment of work means: which rows, which keys.
@@ -76,7 +78,8 @@ __device__ __forceinline__ XFwdUnit x_fwd_unit(const XFwdParams& p, const XSeg& 
 template <bool kBF16, int kD>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ XFwdParams p) {
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+                 const __grid_constant__ XFwdParams p) {
     constexpr int kAtoms = kD / 64;
     constexpr int kOperandBytes = kAtoms * kHalfBytes;
     extern __shared__ uint8_t smem_raw[];
@@ -85,7 +88,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const uint32_t sQ = smem_u32(smem);
     const uint32_t sK = sQ + 2 * kTileBytes;
     const uint32_t sV = sK + 2 * kTileBytes;
-    XFwdCtl* ctl = reinterpret_cast<XFwdCtl*>(smem + 6 * kTileBytes);
+    XFwdCtl* ctl = reinterpret_cast<XFwdCtl*>(smem + 6 * kTileBytes + kSoftmaxWarps * kXStageBytes);
     volatile int* s_abort = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -119,6 +122,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         tma_prefetch_desc(&tm_q);
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
+        tma_prefetch_desc(&tm_o);
     }
     tc_fence_before();
     __syncthreads();
@@ -296,7 +300,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 if (!ok) break;
                 if ((w0 & w1) != ~0ull) {
                     x_zero_rows<kD>(smem + 4 * kTileBytes + st * kTileBytes, w0, w1, lane);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    fence_proxy_async_shared();
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->v_clean[st]));
@@ -434,36 +438,35 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 continue;
             }
             const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;  // (no key at all: zeros, LSE -inf)
-            uint16_t* orow = p.out + (w.b * p.o_sb + head * p.o_sh + row * p.o_ss);
+            uint8_t* stage = smem + 6 * kTileBytes + warp * kXStageBytes;
+            const bool zero = n <= 0 || !(l_sum > 0.0f);
+            const int row_w = (tile - g * p.mt) * kTileM + quarter * 32;  // first of the warp's rows
 #pragma unroll
-            for (int b = 0; b < kD / 32; ++b) {
-                uint32_t o[32];
-                tmem_ld32(tO + b * 32, o);
-                tc_wait_ld();
-                tmem_ld_fence(o);
-                if (n <= 0 || !(l_sum > 0.0f)) {
+            for (int cb = 0; cb < kD / 64; ++cb) {
+                if (lane == 0) tma_store_wait_read();  // (the staging memory is free again)
+                __syncwarp();
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = 0u;
-                }
-                if (in_range) {
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t o[32];
+                    tmem_ld32(tO + cb * 64 + b * 32, o);
+                    tc_wait_ld();
+                    tmem_ld_fence(o);
+                    if (zero) {
 #pragma unroll
-                    for (int v4 = 0; v4 < 4; ++v4) {
-                        uint4 q4;
-                        uint32_t* wp = reinterpret_cast<uint32_t*>(&q4);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float a = __uint_as_float(o[v4 * 8 + 2 * x]) * inv;
-                            const float b2 = __uint_as_float(o[v4 * 8 + 2 * x + 1]) * inv;
-                            wp[x] = kBF16 ? pack_bf16x2(a, b2) : pack_f16x2(a, b2);
-                        }
-                        *reinterpret_cast<uint4*>(orow + b * 32 + v4 * 8) = q4;
+                        for (int x = 0; x < 32; ++x) o[x] = 0u;
                     }
+                    x_stage32<kBF16>(stage, lane, b, o, inv);
                 }
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0 && g < p.group && row_w < p.sq)
+                    tma_store_5d(&tm_o, smem_u32(stage), cb * 64, row_w, head, w.b, 0);
             }
             if (in_range && p.lse != nullptr)
                 p.lse[(static_cast<long long>(w.b) * p.hkv * p.group + head) * p.sq + row] =
                     l_sum > 0.0f ? m_ref * p.scale + logf(l_sum) : -INFINITY;
         }
+        if (lane == 0) tma_store_wait();
     }
     tc_fence_before();
     __syncthreads();
