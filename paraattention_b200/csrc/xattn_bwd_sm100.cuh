@@ -2,22 +2,29 @@
 //   dP = do v^T,  dS = P * (dP - delta),  dq = s dS k,  dk = s dS^T q,  dv = P^T do.
 //
 // Two passes of ONE kernel: the query pass (kKeys = false) owns tiles of 128 query rows and walks
-// the key tiles for dq; the key pass (kKeys = true) owns tiles of 128 keys and walks the query
-// tiles (of every head that shares the key head, and of every batch entry that shares the keys)
-// for dk and dv. In both, the owned pair (X, Y) = (q, do) or (k, v) stays in shared memory, the
-// other pair (Z, W) = (k, v) or (q, do) streams through a two-stage ring, and per step
-//   T1 = X Z^T, T2 = Y W^T                (tensor core, into TMEM)
-//   P = 2^(T1 sl - lse'), dS = P (T2 - delta)   (one thread per owned row and half of the columns)
+// the keys for dq; the key pass (kKeys = true) owns tiles of 128 keys and walks the queries (of every
+// head that shares the key head, and of every batch entry that shares the keys) for dk and dv. In
+// both, the owned pair (X, Y) = (q, do) or (k, v) stays in shared memory, the other pair (Z, W) =
+// (k, v) or (q, do) streams through a ring in blocks of 64 rows, one block a step, and per step
+//   T1 = X Z^T, T2 = Y W^T                (tensor core, 128 x 64, into TMEM)
+//   P = 2^(T1 sl - lse'), dS = P (T2 - delta)   (one thread per owned row and 32 columns)
 //   A1 += dS Z  [, A2 += P W in the key pass]   (tensor core, dS and P as TMEM operands)
 // so dS and P never leave TMEM and are never transposed: the key pass computes their transposes
 // to begin with. The price is that S and dP are computed twice (7 products instead of 5); what it
 // buys is no atomics (sums in a fixed order), no fp32 dq traffic, and each gradient written once.
 //
-// As in the forward kernel a step is run as two halves of the streamed rows (columns of T), each
-// with its own chain T1, T2 -> elementwise -> A: warps 0-3 serve half 0, warps 4-7 half 1, and while one
-// half is in its elementwise phase the tensor core works on the other. TMEM columns: T1 [0,128),
-// T2 [128,256), A1 [256, 256 + D), A2 [256 + D, 256 + 2 D); dS overwrites T2, P overwrites T1.
-// CTAs are persistent and the roles run ahead across units (xattn_sm100.cuh divides the work).
+// Steps alternate between two T buffers, each with its own chain T -> elementwise -> A -> next T: while
+// one is in its elementwise phase the tensor core works on the other. What was measured on the way
+// (16380 queries x 512 keys x 40 heads, cycles per 128 rows, key pass): 8 elementwise warps with 64
+// columns per thread and a ring of two 128-row stages 4600, the tensor core waiting 1600 of them for
+// loads; 16 warps and a ring of four 64-row stages, which are released - and asked for again - half
+// a tile earlier, hide both. The bound then is shared memory: operand fetches of the N = 64 products
+// and the TMA writes are 320 KB per 128 rows of the key pass, 2560 cycles at 128 bytes per cycle.
+//
+// Warps 0-15 elementwise (0-7 even steps, 8-15 odd ones), 16 MMA issuer, 17 TMA producer, 18 clears
+// masked rows of K. TMEM columns: T1 [0,128), T2 [128,256) - 64 per buffer -, A1 [256, 256 + D), A2
+// [256 + D, 256 + 2 D); dS overwrites T2, P overwrites T1. CTAs are persistent and the roles run ahead
+// across units (xattn_sm100.cuh divides the work).
 //
 // What is rounded: P and dS to the tensors' 16-bit type, as operands of a 16-bit product (their
 // relative error, half an ulp, averages out over the sum); everything else is fp32.
@@ -27,15 +34,24 @@
 
 namespace pa {
 
+constexpr int kXBwdSoftWarps = 16;
+constexpr int kXBwdMmaWarp = 16, kXBwdTmaWarp = 17, kXBwdCleanWarp = 18;
+constexpr int kXBwdThreads = 640;
+constexpr int kXStep = 64;                       // streamed rows per step
+constexpr int kXStages = 4;                      // ring of steps
+constexpr int kXAtomBytes = kXStep * 128;        // 64 rows x 64 elements
+constexpr int kXSlotBytes = 2 * kXAtomBytes;     // a Z or W block (head_dim 64 fills half of it)
+
 struct XBwdParams {
     int batch, kv_batch, hkv, group, sq, skv;
     int mt, kt;       // 128-row tiles of the queries / of the keys
+    int mb;           // 64-row blocks of the queries
     float scale, scale_log2;
-    uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv
+    uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv (the joining kernel's)
     long long g_sb[2], g_sh[2], g_ss[2];
-    // [B][Hq][mt * 128] (lse * log2 e, delta); rows behind the last query, and rows without any key, have
-    // (+inf, 0), which makes their P zero
-    const float2* stats;
+    // [B][Hq][2 mt blocks][-lse * log2 e, -delta][64 rows]; rows behind the last query, and rows without
+    // any key, have (-inf, 0), which makes their P zero
+    const float* stats;
     const unsigned long long* words;
     const int* extent;
     XSched sched;
@@ -46,17 +62,24 @@ struct XBwdParams {
 
 struct XBwdCtl {
     uint64_t xy_full, xy_empty;
-    uint64_t zw_full[2], zw_empty[2], z_clean[2];
-    uint64_t t_full[2];   // T1 and T2 of a half are in TMEM
-    uint64_t p_full[2];   // dS and P of a half are in TMEM (128 arrivals)
+    uint64_t zw_full[kXStages], zw_empty[kXStages], z_clean[kXStages];
+    uint64_t t_full[2];   // T1 and T2 of a buffer are in TMEM
+    uint64_t p_full[2];   // dS and P of a buffer are in TMEM (one arrival per warp)
     uint64_t acc_done;    // A1, A2 of a segment are complete
-    uint64_t acc_free;    // the epilogue has read them (256 arrivals)
+    uint64_t acc_free;    // the epilogue has read them (one arrival per warp)
     uint64_t teardown;
     uint32_t tmem_base;
     int abort;
 };
-constexpr int kXBwdStatBytes = 2 * kTileN * 8;
-constexpr int kXBwdSmemBytes = 1024 + 6 * kTileBytes + kXBwdStatBytes + 512;
+// Behind the operands: the query pass's staging of dq (8 warps; the key pass stages dk and dv in the
+// memory of the owned tiles, whose segments are long enough for that not to matter), or the key
+// pass's ring of row statistics.
+constexpr int kXBwdExtraBytes = 8 * kXStageBytes;
+// (... and, behind it, a block of zeros for the tiles of keys that no query sees: the owned tiles' memory
+// may hold the next segment's by then)
+constexpr int kXBwdZeroOffset = 4096;
+static_assert(kXStages * kXStep * 8 <= kXBwdZeroOffset && kXBwdZeroOffset + kXStageBytes <= kXBwdExtraBytes, "both fit");
+constexpr int kXBwdSmemBytes = 1024 + 6 * kTileBytes + kXBwdExtraBytes + 512;
 static_assert(sizeof(XBwdCtl) <= 512, "control block too large");
 static_assert(kXBwdSmemBytes <= 232448, "shared memory");
 
@@ -66,7 +89,7 @@ struct XBwdUnit {
     int t0, t1;
 };
 struct XBwdStep {
-    int b, head, tile;  // streamed tile
+    int b, head, block;  // streamed 64-row block
 };
 
 template <bool kKeys>
@@ -80,25 +103,25 @@ __device__ __forceinline__ XBwdUnit x_bwd_unit(const XBwdParams& p, const XSeg& 
     u.b = x / heads;
     u.t0 = g.t0;
     u.t1 = g.t1;
-    if (!kKeys && p.extent != nullptr) {  // key tiles behind the last key that takes part
-        const int n = (__ldg(p.extent + u.b) + kTileN - 1) / kTileN;
+    if (!kKeys && p.extent != nullptr) {  // blocks behind the last key that takes part
+        const int n = (__ldg(p.extent + u.b) + kXStep - 1) / kXStep;
         u.t1 = min(u.t1, n);
         u.t0 = min(u.t0, u.t1);
     }
     return u;
 }
-// Key pass: steps run over (batch entries that share the keys, heads of the group, query tiles).
+// Key pass: steps run over (batch entries that share the keys, heads of the group, query blocks).
 template <bool kKeys>
 __device__ __forceinline__ XBwdStep x_bwd_step(const XBwdParams& p, const XBwdUnit& u, int step) {
     XBwdStep s;
     if (!kKeys) {
         s.b = p.kv_batch == 1 ? 0 : u.b;
         s.head = u.head / p.group;
-        s.tile = step;
+        s.block = step;
         return s;
     }
-    const int m = step / p.mt;
-    s.tile = step - m * p.mt;
+    const int m = step / p.mb;
+    s.block = step - m * p.mb;
     const int bb = m / p.group;
     s.head = u.head * p.group + (m - bb * p.group);
     s.b = p.kv_batch == 1 ? bb : u.b;
@@ -109,7 +132,7 @@ __device__ __forceinline__ XBwdStep x_bwd_step(const XBwdParams& p, const XBwdUn
 template <bool kKeys>
 __device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u, int step) {
     if (!kKeys || p.extent == nullptr) return step;
-    const int per_b = p.group * p.mt;
+    const int per_b = p.group * p.mb;
     while (step < u.t1) {
         const int b = p.kv_batch == 1 ? step / per_b : u.b;
         if (u.tile * kTileN < __ldg(p.extent + b)) return step;
@@ -120,9 +143,10 @@ __device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u
 }
 
 template <bool kBF16, int kD, bool kKeys>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kXBwdThreads, 1)
 xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y,
                  const __grid_constant__ CUtensorMap tm_z, const __grid_constant__ CUtensorMap tm_w,
+                 const __grid_constant__ CUtensorMap tm_g0, const __grid_constant__ CUtensorMap tm_g1,
                  const __grid_constant__ XBwdParams p) {
     constexpr int kAtoms = kD / 64;
     constexpr int kOperandBytes = kAtoms * kHalfBytes;
@@ -130,9 +154,9 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-    const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sX + 4 * kTileBytes;
-    float2* stat = reinterpret_cast<float2*>(smem + 6 * kTileBytes);  // [stage][128], key pass
-    XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + 6 * kTileBytes + kXBwdStatBytes);
+    const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sZ + kXStages * kXSlotBytes;
+    float* stat = reinterpret_cast<float*>(smem + 6 * kTileBytes);  // [stage][2][64], key pass
+    XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + 6 * kTileBytes + kXBwdExtraBytes);
     volatile int* s_abort = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -141,28 +165,37 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     if (ctl->abort != 0) return;
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&ctl->xy_full), 1);
-        mbar_init(smem_u32(&ctl->xy_empty), 1);
-        for (int s = 0; s < 2; ++s) {
+        mbar_init(smem_u32(&ctl->xy_empty), kKeys ? kXBwdSoftWarps : 1);
+        for (int s = 0; s < kXStages; ++s) {
             mbar_init(smem_u32(&ctl->zw_full[s]), 1);
             mbar_init(smem_u32(&ctl->zw_empty[s]), 1);
             mbar_init(smem_u32(&ctl->z_clean[s]), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
             mbar_init(smem_u32(&ctl->t_full[s]), 1);
-            mbar_init(smem_u32(&ctl->p_full[s]), 128);
+            mbar_init(smem_u32(&ctl->p_full[s]), kXBwdSoftWarps / 2);
         }
         mbar_init(smem_u32(&ctl->acc_done), 1);
-        mbar_init(smem_u32(&ctl->acc_free), 256);
+        mbar_init(smem_u32(&ctl->acc_free), kXBwdSoftWarps);
         mbar_init(smem_u32(&ctl->teardown), 1);
         mbar_init_fence();
     }
-    if (warp == kMmaWarp) {
+    if (kKeys) {
+        for (int i = threadIdx.x; i < kXStageBytes / 16; i += kXBwdThreads)
+            reinterpret_cast<uint4*>(smem + 6 * kTileBytes + kXBwdZeroOffset)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_shared();
+    }
+    if (warp == kXBwdMmaWarp) {
         tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
         tmem_relinquish();
     }
-    if (warp == kTmaWarp && lane == 0) {
+    if (warp == kXBwdTmaWarp && lane == 0) {
         tma_prefetch_desc(&tm_x);
         tma_prefetch_desc(&tm_y);
         tma_prefetch_desc(&tm_z);
         tma_prefetch_desc(&tm_w);
+        tma_prefetch_desc(&tm_g0);
+        if (kKeys) tma_prefetch_desc(&tm_g1);
     }
     tc_fence_before();
     __syncthreads();
@@ -174,7 +207,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 
     XCursor cursor(p.sched);
     XSeg seg;
-    if (warp == kTmaWarp) {
+    if (warp == kXBwdTmaWarp) {
         // =============================== TMA producer ======================================
         if (lane == 0) {
             bool ok = true;
@@ -194,22 +227,23 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 }
                 for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
                     const XBwdStep s = x_bwd_step<kKeys>(p, u, st);
-                    const int sg = j & 1;
+                    const int sg = j % kXStages;
                     const uint32_t bz = smem_u32(&ctl->zw_full[sg]);
-                    if (j >= 2) ok = mbar_wait(smem_u32(&ctl->zw_empty[sg]), ((j >> 1) & 1) ^ 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                    if (j >= kXStages)
+                        ok = mbar_wait(smem_u32(&ctl->zw_empty[sg]), ((j / kXStages) & 1) ^ 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
                     if (!ok) break;
-                    mbar_expect_tx(bz, 2 * kOperandBytes + (kKeys ? kTileN * 8 : 0));
+                    mbar_expect_tx(bz, 2 * kAtoms * kXAtomBytes + (kKeys ? kXStep * 8 : 0));
 #pragma unroll
                     for (int h = 0; h < kAtoms; ++h) {
-                        tma_load_5d(sZ + sg * kTileBytes + h * kHalfBytes, &tm_z, bz, h * 64, s.tile * kTileN, s.head, s.b, 0);
-                        tma_load_5d(sW + sg * kTileBytes + h * kHalfBytes, &tm_w, bz, h * 64, s.tile * kTileN, s.head, s.b, 0);
+                        tma_load_5d(sZ + sg * kXSlotBytes + h * kXAtomBytes, &tm_z, bz, h * 64, s.block * kXStep, s.head, s.b, 0);
+                        tma_load_5d(sW + sg * kXSlotBytes + h * kXAtomBytes, &tm_w, bz, h * 64, s.block * kXStep, s.head, s.b, 0);
                     }
                     if (kKeys) {
-                        const float2* src = p.stats + ((static_cast<long long>(s.b) * p.hkv * p.group + s.head) * p.mt + s.tile) * kTileN;
+                        const float* src = p.stats + ((static_cast<long long>(s.b) * p.hkv * p.group + s.head) * (2 * p.mt) + s.block) * (2 * kXStep);
                         asm volatile(
                             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                smem_u32(stat + sg * kTileN)),
-                            "l"(src), "r"(kTileN * 8), "r"(bz)
+                                smem_u32(stat + sg * 2 * kXStep)),
+                            "l"(src), "r"(kXStep * 8), "r"(bz)
                             : "memory");
                     }
                 }
@@ -220,46 +254,48 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 volatile int* no_abort = &none;
                 if (n_seg > 0) mbar_wait(smem_u32(&ctl->xy_full), (n_seg - 1) & 1, no_abort, nullptr, 10000000ull, 0);
                 mbar_wait(smem_u32(&ctl->xy_full), n_seg & 1, no_abort, nullptr, 10000000ull, 0);
-                for (int jj = (j > 2 ? j - 2 : 0); jj <= j; ++jj)
-                    mbar_wait(smem_u32(&ctl->zw_full[jj & 1]), (jj >> 1) & 1, no_abort, nullptr, 10000000ull, 0);
+                for (int jj = (j > kXStages ? j - kXStages : 0); jj <= j; ++jj)
+                    mbar_wait(smem_u32(&ctl->zw_full[jj % kXStages]), (jj / kXStages) & 1, no_abort, nullptr, 10000000ull, 0);
             }
         }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == kXBwdMmaWarp) {
         // =============================== MMA issuer ========================================
         constexpr uint32_t idesc_t = make_idesc_f16(kBF16, false, kTileM, 64);
         constexpr uint32_t idesc_a = make_idesc_f16(kBF16, true, kTileM, kD);
         const uint32_t leader = elect_one() ? 1u : 0u;
         // K-major descriptors (T1, T2) and MN-major descriptors (the same tiles as B operands of A1, A2)
-        const uint64_t dk0 = smem_desc_sw128(sX, 16, 1024), dm0 = smem_desc_sw128(sZ, kHalfBytes, 1024);
+        const uint64_t dk0 = smem_desc_sw128(sX, 16, 1024), dm0 = smem_desc_sw128(sZ, kXAtomBytes, 1024);
         const uint32_t hi_k = static_cast<uint32_t>(dk0 >> 32), hi_m = static_cast<uint32_t>(dm0 >> 32);
         const uint32_t lo_x = static_cast<uint32_t>(dk0), lo_y = lo_x + (kTileBytes >> 4);
-        const uint32_t lo_z = static_cast<uint32_t>(smem_desc_sw128(sZ, 16, 1024)), lo_w = lo_z + (2 * kTileBytes >> 4);
-        const uint32_t lo_zm = static_cast<uint32_t>(dm0), lo_wm = lo_zm + (2 * kTileBytes >> 4);
-        auto issue_t = [&](int sg, int half) {
-            const uint32_t zo = (sg * kTileBytes + half * 64 * 128) >> 4;
+        const uint32_t lo_z = static_cast<uint32_t>(smem_desc_sw128(sZ, 16, 1024)), lo_w = lo_z + (kXStages * kXSlotBytes >> 4);
+        const uint32_t lo_zm = static_cast<uint32_t>(dm0), lo_wm = lo_zm + (kXStages * kXSlotBytes >> 4);
+        // T of the step in ring slot sg into buffer t
+        auto issue_t = [&](int sg, int t) {
+            const uint32_t zo = (sg * kXSlotBytes) >> 4;
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
-                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                tc_mma_ss_elect(tmem + kColT1 + half * 64, lo_x + off, hi_k, lo_z + zo + off, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                const uint32_t ao = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4, bo = ((ks >> 2) * kXAtomBytes + (ks & 3) * 32) >> 4;
+                tc_mma_ss_elect(tmem + kColT1 + t * 64, lo_x + ao, hi_k, lo_z + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
             }
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
-                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-                tc_mma_ss_elect(tmem + kColT2 + half * 64, lo_y + off, hi_k, lo_w + zo + off, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                const uint32_t ao = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4, bo = ((ks >> 2) * kXAtomBytes + (ks & 3) * 32) >> 4;
+                tc_mma_ss_elect(tmem + kColT2 + t * 64, lo_y + ao, hi_k, lo_w + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
             }
-            tc_commit_elect(smem_u32(&ctl->t_full[half]), leader);
+            tc_commit_elect(smem_u32(&ctl->t_full[t]), leader);
         };
-        auto issue_a = [&](int sg, int half, bool acc) {
-            const uint32_t so = (sg * kTileBytes + half * 64 * 128) >> 4;
+        // (16 streamed rows a k-step; their dS / P are 8 packed columns, 32 columns of T packed into 16)
+        auto issue_a = [&](int sg, int t, bool acc) {
+            const uint32_t so = (sg * kXSlotBytes) >> 4;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-                tc_mma_ts_elect(tmem + kColA1, tmem + kColT2 + half * 64 + ks * 8, lo_zm + so + ((ks * 16 * 128) >> 4), hi_m,
-                                idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
+                tc_mma_ts_elect(tmem + kColA1, tmem + kColT2 + t * 64 + (ks >> 1) * 32 + (ks & 1) * 8, lo_zm + so + ((ks * 16 * 128) >> 4),
+                                hi_m, idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
             if (kKeys) {
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
-                    tc_mma_ts_elect(tmem + kColA2, tmem + kColT1 + half * 64 + ks * 8, lo_wm + so + ((ks * 16 * 128) >> 4), hi_m,
-                                    idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
+                    tc_mma_ts_elect(tmem + kColA2, tmem + kColT1 + t * 64 + (ks >> 1) * 32 + (ks & 1) * 8,
+                                    lo_wm + so + ((ks * 16 * 128) >> 4), hi_m, idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
             }
         };
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
@@ -267,7 +303,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             return __all_sync(0xffffffffu, r);
         };
         auto wait_zw = [&](int j) -> bool {
-            return wait(clean ? &ctl->z_clean[j & 1] : &ctl->zw_full[j & 1], (j >> 1) & 1);
+            return wait(clean ? &ctl->z_clean[j % kXStages] : &ctl->zw_full[j % kXStages], (j / kXStages) & 1);
         };
         bool ok = true, issued = false;
         int j = 0, n_seg = 0;  // steps, segments with steps
@@ -275,41 +311,41 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
             if (st >= u.t1) continue;
-            int nx = x_bwd_live<kKeys>(p, u, st + 1);
+            // T runs two steps ahead of A
+            int ahead = x_bwd_live<kKeys>(p, u, st + 1);
             ok = wait(&ctl->xy_full, n_seg & 1) && wait_zw(j);
             if (!ok) break;
             tc_fence_after();
             issued = true;
-            issue_t(j & 1, 0);
-            issue_t(j & 1, 1);
-            if (nx >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
-            bool first = true;
-            while (true) {
-                const bool more = nx < u.t1;
-                int nx2 = nx;
-                if (more) {
-                    nx2 = x_bwd_live<kKeys>(p, u, nx + 1);
-                    ok = wait_zw(j + 1);
-                    if (!ok) break;
-                }
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    ok = wait(&ctl->p_full[half], j & 1);
-                    // (the accumulators of the segment before have been read by the epilogue)
-                    if (ok && first && half == 0 && n_seg > 0) ok = wait(&ctl->acc_free, (n_seg - 1) & 1);
+            issue_t(j % kXStages, j & 1);
+            bool two = ahead < u.t1;
+            if (two) {
+                ok = wait_zw(j + 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_t((j + 1) % kXStages, (j + 1) & 1);
+                ahead = x_bwd_live<kKeys>(p, u, ahead + 1);
+            }
+            if (!kKeys && ahead >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
+            int left = two ? 2 : 1;  // steps whose T is issued and whose A is not
+            for (bool first = true; left > 0; first = false, ++j) {
+                ok = wait(&ctl->p_full[j & 1], (j >> 1) & 1);
+                // (the accumulators of the segment before have been read by the epilogue)
+                if (ok && first && n_seg > 0) ok = wait(&ctl->acc_free, (n_seg - 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_a(j % kXStages, j & 1, !first);
+                tc_commit_elect(smem_u32(&ctl->zw_empty[j % kXStages]), leader);
+                --left;
+                if (ahead < u.t1) {
+                    ok = wait_zw(j + 2);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_a(j & 1, half, !first || half > 0);
-                    if (half == 1) tc_commit_elect(smem_u32(&ctl->zw_empty[j & 1]), leader);
-                    if (more) issue_t((j + 1) & 1, half);
+                    issue_t((j + 2) % kXStages, j & 1);
+                    ++left;
+                    ahead = x_bwd_live<kKeys>(p, u, ahead + 1);
+                    if (!kKeys && ahead >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
                 }
-                if (!ok) break;
-                if (more && nx2 >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
-                ++j;
-                first = false;
-                if (!more) break;
-                st = nx;
-                nx = nx2;
             }
             if (!ok) break;
             tc_commit_elect(smem_u32(&ctl->acc_done), leader);
@@ -321,7 +357,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             tc_commit_elect(smem_u32(&ctl->teardown), leader);
             mbar_wait(smem_u32(&ctl->teardown), 0, no_abort, nullptr, 100000000ull, 0);
         }
-    } else if (warp == kTmaWarp + 1 && clean) {
+    } else if (warp == kXBwdCleanWarp && clean) {
         // =============================== masked rows of K ==================================
         bool ok = true;
         int j = 0;
@@ -329,27 +365,27 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             const unsigned long long* row = p.words + static_cast<long long>(u.b) * n_words;
             for (int t = u.t0; t < u.t1; ++t, ++j) {
-                const int sg = j & 1;
-                const unsigned long long w0 = x_key_word(row, p.skv, t, 0), w1 = x_key_word(row, p.skv, t, 1);
-                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->zw_full[sg]), (j >> 1) & 1, s_abort, p.status, limit,
+                const int sg = j % kXStages;
+                const unsigned long long word = x_key_word(row, p.skv, t);
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->zw_full[sg]), (j / kXStages) & 1, s_abort, p.status, limit,
                                                        PA_DEV_TIMEOUT_PIPE));
                 if (!ok) break;
-                if ((w0 & w1) != ~0ull) {
-                    x_zero_rows<kD>(smem + 2 * kTileBytes + sg * kTileBytes, w0, w1, lane);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                if (word != ~0ull) {
+                    x_zero_rows<kD>(smem + 2 * kTileBytes + sg * kXSlotBytes, kXAtomBytes, word, lane);
+                    fence_proxy_async_shared();
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->z_clean[sg]));
             }
         }
-    } else if (warp < kSoftmaxWarps) {
+    } else if (warp < kXBwdSoftWarps) {
         // =============================== elementwise + epilogue ============================
-        const int quarter = warp & 3, half = warp >> 2;
+        const int quarter = warp & 3, piece = warp >> 2, buf = piece >> 1;  // my lanes; my 32 columns; their T buffer
         const int row_in_tile = quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t t1 = tmem + lane_base + kColT1 + half * 64, t2 = tmem + lane_base + kColT2 + half * 64;
-        const float sl = p.scale_log2;
-        const float2 sl2 = make_float2(sl, sl);
+        const uint32_t t1 = tmem + lane_base + kColT1 + piece * 32, t2 = tmem + lane_base + kColT2 + piece * 32;
+        // (dS and P of my 32 columns are packed into the first 16 of them: no other warp reads or writes there)
+        const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
         bool ok = true;
         int j = 0, n_seg = 0;
         while (ok && cursor.next(p.sched, seg)) {
@@ -357,64 +393,70 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             int st = x_bwd_live<kKeys>(p, u, u.t0);
             const bool any = st < u.t1;
             const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
-            float2 mine = make_float2(0.f, 0.f);
-            if (!kKeys)
-                mine = __ldg(p.stats + (static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt * kTileM + row);
-            for (; st < u.t1 && ok; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
-                unsigned long long word = ~0ull;  // query pass: my half's keys; key pass: all or nothing
+            float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
+            if (!kKeys) {
+                const float* r = p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * (2 * p.mt) + (row >> 6)) * (2 * kXStep) + (row & 63);
+                neg.x = neg.y = __ldg(r);
+                dl.x = dl.y = __ldg(r + kXStep);
+            }
+            for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
+                if ((j & 1) != buf) continue;
+                uint32_t live = 0xffffffffu;  // query pass: my columns' keys; key pass: all or nothing
                 if (!kKeys) {
-                    word = x_key_word(p.words != nullptr ? p.words + static_cast<long long>(u.b) * n_words : nullptr, p.skv, st, half);
+                    live = static_cast<uint32_t>(
+                        x_key_word(p.words != nullptr ? p.words + static_cast<long long>(u.b) * n_words : nullptr, p.skv, st) >>
+                        ((piece & 1) * 32));
                 } else if (p.words != nullptr) {
                     const int b = x_bwd_step<kKeys>(p, u, st).b;
-                    if (row >= p.skv || ((__ldg(p.words + static_cast<long long>(b) * n_words + (row >> 6)) >> (row & 63)) & 1ull) == 0) word = 0ull;
+                    if (row >= p.skv || ((__ldg(p.words + static_cast<long long>(b) * n_words + (row >> 6)) >> (row & 63)) & 1ull) == 0) live = 0u;
                 } else if (row >= p.skv) {
-                    word = 0ull;
+                    live = 0u;
                 }
-                const bool plain = __all_sync(0xffffffffu, word == ~0ull);
+                const bool plain = __all_sync(0xffffffffu, live == 0xffffffffu);
                 if (kKeys)  // (the step's statistics are in shared memory: already true when t_full is)
-                    ok = mbar_wait(smem_u32(&ctl->zw_full[j & 1]), (j >> 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
-                ok = mbar_wait(smem_u32(&ctl->t_full[half]), j & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE) && ok;
+                    ok = mbar_wait(smem_u32(&ctl->zw_full[j % kXStages]), (j / kXStages) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                ok = mbar_wait(smem_u32(&ctl->t_full[buf]), (j >> 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE) && ok;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const float4* col = reinterpret_cast<const float4*>(stat + (j & 1) * kTileN + half * 64);
+                uint32_t a[32], d[32];
+                tmem_ld32(t1, a);
+                tmem_ld32(t2, d);
+                tc_wait_ld();
+                tmem_ld_fence(a);
+                tmem_ld_fence(d);
+                const float4* cl = reinterpret_cast<const float4*>(stat + (j % kXStages) * 2 * kXStep + (piece & 1) * 32);
+                uint32_t pp[16], ds[16];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t a[32], d[32], pp[16], ds[16];
-                    tmem_ld32(t1 + c * 32, a);
-                    tmem_ld32(t2 + c * 32, d);
-                    tc_wait_ld();
-                    tmem_ld_fence(a);
-                    tmem_ld_fence(d);
-                    const uint32_t live = static_cast<uint32_t>(word >> (c * 32));
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float2 neg, dl;
-                        if (kKeys) {
-                            const float4 s4 = col[c * 16 + (i >> 1)];
-                            neg = make_float2(-s4.x, -s4.z);
-                            dl = make_float2(-s4.y, -s4.w);
-                        } else {
-                            neg = make_float2(-mine.x, -mine.x);
-                            dl = make_float2(-mine.y, -mine.y);
-                        }
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), sl2, neg);
-                        float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                        const float2 t = __fadd2_rn(make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])), dl);
-                        float2 s = __fmul2_rn(e, t);
-                        if (!plain) {
-                            if (((live >> i) & 1u) == 0) e.x = s.x = 0.f;
-                            if (((live >> (i + 1)) & 1u) == 0) e.y = s.y = 0.f;
-                        }
-                        if (kKeys) pp[i >> 1] = kBF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
-                        ds[i >> 1] = kBF16 ? pack_bf16x2(s.x, s.y) : pack_f16x2(s.x, s.y);
+                for (int i = 0; i < 32; i += 4) {
+                    float2 ng[2] = {neg, neg}, dt[2] = {dl, dl};
+                    if (kKeys) {
+                        const float4 l4 = cl[i >> 2], d4 = cl[(i >> 2) + kXStep / 4];
+                        ng[0] = make_float2(l4.x, l4.y);
+                        ng[1] = make_float2(l4.z, l4.w);
+                        dt[0] = make_float2(d4.x, d4.y);
+                        dt[1] = make_float2(d4.z, d4.w);
                     }
-                    tmem_st16(t2 + c * 16, ds);
-                    if (kKeys) tmem_st16(t1 + c * 16, pp);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int c = i + 2 * y;
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), sl2, ng[y]);
+                        float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                        float2 s = __fmul2_rn(e, __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dt[y]));
+                        if (!plain) {
+                            if (((live >> c) & 1u) == 0) e.x = s.x = 0.f;
+                            if (((live >> (c + 1)) & 1u) == 0) e.y = s.y = 0.f;
+                        }
+                        if (kKeys) pp[c >> 1] = kBF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+                        ds[c >> 1] = kBF16 ? pack_bf16x2(s.x, s.y) : pack_f16x2(s.x, s.y);
+                    }
                 }
+                tmem_st16(t2, ds);
+                if (kKeys) tmem_st16(t1, pp);
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(smem_u32(&ctl->p_full[half]));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->p_full[buf]));
             }
             if (any && ok) {
                 ok = mbar_wait(smem_u32(&ctl->acc_done), n_seg & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
@@ -423,57 +465,67 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            // Key pass: warps 0-3 write dk, warps 4-7 dv. Query pass: each half of the warps writes half
-            // of dq's columns.
-            const int which = kKeys ? half : 0;
-            constexpr int kBlocks = kKeys ? kD / 32 : kD / 64;
-            const int block0 = kKeys ? 0 : half * kBlocks;
-            const uint32_t ta = tmem + lane_base + (which ? kColA2 : kColA1);
-            const float factor = which ? 1.0f : p.scale;
-            const bool in_range = row < (kKeys ? p.skv : p.sq);
-            uint16_t* grow = p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]);
-            float4* part = reinterpret_cast<float4*>(p.part) +
-                           (static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) * kTileM + row_in_tile;
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const int blk = block0 + b;
-                uint32_t o[32];
-                tmem_ld32(ta + blk * 32, o);
-                tc_wait_ld();
-                tmem_ld_fence(o);
-                if (!any) {
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+            // Each warp writes 32 rows x 64 columns: the key pass's warps those of dk and dv, the query pass's
+            // first warps those of dq.
+            const int which = kKeys ? piece / (kD / 64) : 0;
+            const int cb = kKeys ? piece % (kD / 64) : piece;  // 64-column block
+            const bool mine = which < 2 && cb < kD / 64;
+            if (kKeys && !any && mine && seg.slot < 0) {
+                const int row_w = u.tile * kTileM + quarter * 32;
+                if (lane == 0 && row_w < p.skv)
+                    tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(smem + 6 * kTileBytes + kXBwdZeroOffset), cb * 64, row_w, u.head, u.b, 0);
+            } else if (mine) {
+                const uint32_t ta = tmem + lane_base + (which ? kColA2 : kColA1) + cb * 64;
+                const int row_w = u.tile * kTileM + quarter * 32;
+                uint8_t* stage = kKeys ? smem + warp * kXStageBytes : smem + 6 * kTileBytes + warp * kXStageBytes;
+                if (seg.slot < 0) {
+                    if (lane == 0) tma_store_wait_read();  // (the staging memory is free again)
+                    __syncwarp();
                 }
-                if (seg.slot >= 0) {
 #pragma unroll
-                    for (int v4 = 0; v4 < 8; ++v4)
-                        __stcg(part + (blk * 8 + v4) * kTileM,
-                               make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
-                                           __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
-                } else if (in_range) {
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t o[32];
+                    tmem_ld32(ta + b * 32, o);
+                    tc_wait_ld();
+                    tmem_ld_fence(o);
+                    if (!any) {
 #pragma unroll
-                    for (int v4 = 0; v4 < 4; ++v4) {
-                        uint32_t q[4];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float f0 = __uint_as_float(o[v4 * 8 + 2 * x]) * factor;
-                            const float f1 = __uint_as_float(o[v4 * 8 + 2 * x + 1]) * factor;
-                            q[x] = kBF16 ? pack_bf16x2(f0, f1) : pack_f16x2(f0, f1);
-                        }
-                        *reinterpret_cast<uint4*>(grow + blk * 32 + v4 * 8) = make_uint4(q[0], q[1], q[2], q[3]);
+                        for (int x = 0; x < 32; ++x) o[x] = 0u;
                     }
+                    if (seg.slot < 0) {
+                        x_stage32<kBF16>(stage, lane, b, o, which ? 1.0f : p.scale);
+                    } else {
+                        float4* part = reinterpret_cast<float4*>(p.part) +
+                                       ((static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) + cb * 16 + b * 8) * kTileM + row_in_tile;
+#pragma unroll
+                        for (int v4 = 0; v4 < 8; ++v4)
+                            __stcg(part + v4 * kTileM,
+                                   make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
+                                               __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
+                    }
+                }
+                if (seg.slot < 0) {
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0 && row_w < (kKeys ? p.skv : p.sq))
+                        tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(stage), cb * 64, row_w, u.head, u.b, 0);
                 }
             }
             if (any) {
                 tc_fence_before();
-                mbar_arrive(smem_u32(&ctl->acc_free));
+                if (kKeys && lane == 0) tma_store_wait_read();  // (then the owned tiles may be replaced)
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&ctl->acc_free));
+                    if (kKeys) mbar_arrive(smem_u32(&ctl->xy_empty));
+                }
             }
         }
+        if (lane == 0) tma_store_wait();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) {
+    if (warp == kXBwdMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
@@ -520,13 +572,13 @@ xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, int grid) {
     }
 }
 
-// stats[b][h][row] = (lse * log2 e, sum_d do * out) for the query rows, (+inf, 0) for rows without
+// stats[b][h][64-row block][0 / 1][64] = -lse * log2 e and -sum_d do * out of the query rows; (-inf, 0) for rows without
 // any key and behind the last one. HBM-bound: one pass over do and out, 16 bytes per lane.
 struct XStatParams {
     const uint16_t *o, *g;  // out, do
     long long o_s[3], g_s[3];
     const float* lse;  // [B][Hq][Sq]
-    float2* stats;     // [B][Hq][padded]
+    float* stats;      // [B][Hq][padded / 64][2][64]
     int batch, heads, sq, padded;
 };
 constexpr int kXStatThreads = 256;
@@ -560,12 +612,14 @@ xattn_stat_kernel(const __grid_constant__ XStatParams p) {
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
         if (at == 0 && idx < n) {
-            float2 r = make_float2(INFINITY, 0.f);
+            float2 r = make_float2(-INFINITY, 0.f);
             if (live) {
                 const float l = __ldg(p.lse + (static_cast<long long>(b) * p.heads + h) * p.sq + s);
-                if (l != -INFINITY) r = make_float2(l * 1.4426950408889634f, dot);
+                if (l != -INFINITY) r = make_float2(l * -1.4426950408889634f, -dot);
             }
-            p.stats[(static_cast<long long>(b) * p.heads + h) * p.padded + s] = r;
+            float* dst = p.stats + (static_cast<long long>(b) * p.heads + h) * p.padded * 2 + (s / kXStep) * (2 * kXStep) + s % kXStep;
+            dst[0] = r.x;
+            dst[kXStep] = r.y;
         }
     }
 }

@@ -293,13 +293,14 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const unsigned long long* row = p.words + static_cast<long long>(w.b) * n_words;
             for (int t = w.lo; t < w.hi && ok; ++t, ++j) {
                 const int st = j & 1;
-                const unsigned long long w0 = x_key_word(row, p.skv, t, 0);
-                const unsigned long long w1 = x_key_word(row, p.skv, t, 1);
+                const unsigned long long w0 = x_key_word(row, p.skv, 2 * t);
+                const unsigned long long w1 = x_key_word(row, p.skv, 2 * t + 1);
                 ok = mbar_wait(smem_u32(&ctl->v_full[st]), (j >> 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if ((w0 & w1) != ~0ull) {
-                    x_zero_rows<kD>(smem + 4 * kTileBytes + st * kTileBytes, w0, w1, lane);
+                    x_zero_rows<kD>(smem + 4 * kTileBytes + st * kTileBytes, kHalfBytes, w0, lane);
+                    x_zero_rows<kD>(smem + 4 * kTileBytes + st * kTileBytes + 64 * 128, kHalfBytes, w1, lane);
                     fence_proxy_async_shared();
                 }
                 __syncwarp();
@@ -325,8 +326,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             bool pre = false;
             int pending = -1;
             for (int i = 0; i < n && ok; ++i, ++j) {
-                const unsigned long long kw0 = x_key_word(mrow, p.skv, w.lo + i, 0);
-                const unsigned long long kw1 = x_key_word(mrow, p.skv, w.lo + i, 1);
+                const unsigned long long kw0 = x_key_word(mrow, p.skv, 2 * (w.lo + i));
+                const unsigned long long kw1 = x_key_word(mrow, p.skv, 2 * (w.lo + i) + 1);
                 const bool plain = (kw0 & kw1) == ~0ull;  // (the same for the whole CTA)
 #pragma unroll
                 for (int c = 0; c < kPieces; ++c) {

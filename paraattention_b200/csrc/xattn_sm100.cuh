@@ -116,29 +116,27 @@ xattn_mask_kernel(const uint8_t* __restrict__ mask, long long batch_stride, int 
     }
 }
 
-// A key tile's word for columns [64 half, 64 half + 64): keys that exist and that the mask keeps.
-__device__ __forceinline__ unsigned long long x_key_word(const unsigned long long* words, int keys, int tile, int half) {
-    const int k0 = tile * kTileN + half * 64;
+// The word of keys [64 block, 64 block + 64): those that exist and that the mask keeps.
+__device__ __forceinline__ unsigned long long x_key_word(const unsigned long long* words, int keys, int block) {
+    const int k0 = block * 64;
     if (k0 >= keys) return 0ull;
     if (words != nullptr) return __ldg(words + (k0 >> 6));
     const int n = keys - k0;
     return n >= 64 ? ~0ull : (1ull << n) - 1ull;
 }
 
-// Zeroes the rows of a loaded key / value tile (two 64-row words, clear bit = row is masked) in
-// shared memory. The products with masked rows are multiplied by zero weights; this keeps
-// infinities and NaN that such rows may hold out of the sums. One whole warp calls.
+// Zeroes the rows of a loaded block of 64 keys or values (clear bit of `word` = row is masked) in shared
+// memory; `base`: its first row, 64-element swizzle atoms atom_stride bytes apart. The products with
+// masked rows are multiplied by zero weights; this keeps infinities and NaN that such rows may hold
+// out of the sums. One whole warp calls.
 template <int kD>
-__device__ __forceinline__ void x_zero_rows(uint8_t* tile, unsigned long long w0, unsigned long long w1, int lane) {
+__device__ __forceinline__ void x_zero_rows(uint8_t* base, int atom_stride, unsigned long long word, int lane) {
     constexpr int kChunks = kD / 8;  // 16-byte chunks per row
     constexpr int kRows = 32 / kChunks;
-    const int chunk = lane % kChunks, sub = lane / kChunks;
-    uint8_t* base = tile + (chunk / 8) * kHalfBytes + (chunk % 8) * 16;
-    for (int r0 = 0; r0 < kTileN; r0 += kRows) {
-        const int r = r0 + sub;
-        const unsigned long long w = r < 64 ? w0 : w1;
-        if (((w >> (r & 63)) & 1ull) == 0) *reinterpret_cast<uint4*>(base + r * 128) = make_uint4(0, 0, 0, 0);
-    }
+    const int chunk = lane % kChunks;
+    uint8_t* at = base + (chunk / 8) * atom_stride + (chunk % 8) * 16;
+    for (int r = lane / kChunks; r < 64; r += kRows)
+        if (((word >> r) & 1ull) == 0) *reinterpret_cast<uint4*>(at + r * 128) = make_uint4(0, 0, 0, 0);
 }
 
 // Writes 32 rows x 64 columns of results, one row per lane (`o`: 64 fp32 values of the lane's row, in two
