@@ -4,8 +4,8 @@
 // Two passes of ONE kernel: the query pass (kKeys = false) owns tiles of 128 query rows and walks
 // the keys for dq; the key pass (kKeys = true) owns tiles of 128 keys and walks the queries (of every
 // head that shares the key head, and of every batch entry that shares the keys) for dk and dv. In
-// both, the owned pair (X, Y) = (q, do) or (k, v) stays in shared memory, the other pair (Z, W) =
-// (k, v) or (q, do) streams through a ring in blocks of 64 rows, one block a step, and per step
+// both, the owned pair (X, Y) = (q, do) or (k, v) stays on the SM, the other pair (Z, W) = (k, v) or
+// (q, do) streams through a ring in blocks of 64 rows, one block a step, and per step
 //   T1 = X Z^T, T2 = Y W^T                (tensor core, 128 x 64, into TMEM)
 //   P = 2^(T1 sl - lse'), dS = P (T2 - delta)   (one thread per owned row and 32 columns)
 //   A1 += dS Z  [, A2 += P W in the key pass]   (tensor core, dS and P as TMEM operands)
@@ -62,6 +62,7 @@ struct XBwdParams {
 
 struct XBwdCtl {
     uint64_t xy_full, xy_empty;
+    uint64_t xt_full;     // query pass: X and Y are in TMEM (one arrival per warp)
     uint64_t zw_full[kXStages], zw_empty[kXStages], z_clean[kXStages];
     uint64_t t_full[2];   // T1 and T2 of a buffer are in TMEM
     uint64_t p_full[2];   // dS and P of a buffer are in TMEM (one arrival per warp)
@@ -151,6 +152,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     constexpr int kAtoms = kD / 64;
     constexpr int kOperandBytes = kAtoms * kHalfBytes;
     constexpr uint32_t kColT1 = 0, kColT2 = 128, kColA1 = 256, kColA2 = 256 + kD;
+    constexpr uint32_t kColX = 384, kColY = 448;  // query pass
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
@@ -165,7 +167,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     if (ctl->abort != 0) return;
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&ctl->xy_full), 1);
-        mbar_init(smem_u32(&ctl->xy_empty), kKeys ? kXBwdSoftWarps : 1);
+        mbar_init(smem_u32(&ctl->xy_empty), kXBwdSoftWarps);
+        mbar_init(smem_u32(&ctl->xt_full), kXBwdSoftWarps);
         for (int s = 0; s < kXStages; ++s) {
             mbar_init(smem_u32(&ctl->zw_full[s]), 1);
             mbar_init(smem_u32(&ctl->zw_empty[s]), 1);
@@ -275,12 +278,14 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
                 const uint32_t ao = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4, bo = ((ks >> 2) * kXAtomBytes + (ks & 3) * 32) >> 4;
-                tc_mma_ss_elect(tmem + kColT1 + t * 64, lo_x + ao, hi_k, lo_z + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                if (kKeys) tc_mma_ss_elect(tmem + kColT1 + t * 64, lo_x + ao, hi_k, lo_z + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                else tc_mma_ts_elect(tmem + kColT1 + t * 64, tmem + kColX + ks * 8, lo_z + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
             }
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
                 const uint32_t ao = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4, bo = ((ks >> 2) * kXAtomBytes + (ks & 3) * 32) >> 4;
-                tc_mma_ss_elect(tmem + kColT2 + t * 64, lo_y + ao, hi_k, lo_w + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                if (kKeys) tc_mma_ss_elect(tmem + kColT2 + t * 64, lo_y + ao, hi_k, lo_w + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                else tc_mma_ts_elect(tmem + kColT2 + t * 64, tmem + kColY + ks * 8, lo_w + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
             }
             tc_commit_elect(smem_u32(&ctl->t_full[t]), leader);
         };
@@ -313,7 +318,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             if (st >= u.t1) continue;
             // T runs two steps ahead of A
             int ahead = x_bwd_live<kKeys>(p, u, st + 1);
-            ok = wait(&ctl->xy_full, n_seg & 1) && wait_zw(j);
+            ok = wait(kKeys ? &ctl->xy_full : &ctl->xt_full, n_seg & 1) && wait_zw(j);
             if (!ok) break;
             tc_fence_after();
             issued = true;
@@ -326,7 +331,6 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 issue_t((j + 1) % kXStages, (j + 1) & 1);
                 ahead = x_bwd_live<kKeys>(p, u, ahead + 1);
             }
-            if (!kKeys && ahead >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
             int left = two ? 2 : 1;  // steps whose T is issued and whose A is not
             for (bool first = true; left > 0; first = false, ++j) {
                 ok = wait(&ctl->p_full[j & 1], (j >> 1) & 1);
@@ -344,7 +348,6 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                     issue_t((j + 2) % kXStages, j & 1);
                     ++left;
                     ahead = x_bwd_live<kKeys>(p, u, ahead + 1);
-                    if (!kKeys && ahead >= u.t1) tc_commit_elect(smem_u32(&ctl->xy_empty), leader);
                 }
             }
             if (!ok) break;
@@ -386,12 +389,46 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         const uint32_t t1 = tmem + lane_base + kColT1 + piece * 32, t2 = tmem + lane_base + kColT2 + piece * 32;
         // (dS and P of my 32 columns are packed into the first 16 of them: no other warp reads or writes there)
         const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-        bool ok = true;
+        // Query pass: brings a segment's X and Y from shared memory to TMEM once its predecessor's products
+        // are done (false: a wait gave up). D / 8 16-byte chunks per row, four of them per warp.
+        int n_copied = 0;
+        auto copy_xy = [&]() -> bool {
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->xy_full), n_copied & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE)))
+                return false;
+            ++n_copied;
+            if (piece * 4 < kD / 8) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint8_t* src = smem + y * kTileBytes + (piece >> 1) * kHalfBytes + row_in_tile * 128;
+                    uint32_t v[16];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(src + (((((piece & 1) << 2) + i) ^ (row_in_tile & 7)) << 4));
+                        v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+                    }
+                    tmem_st16(tmem + lane_base + (y ? kColY : kColX) + piece * 16, v);
+                }
+                tc_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&ctl->xt_full));
+                mbar_arrive(smem_u32(&ctl->xy_empty));
+            }
+            return true;
+        };
+        bool ok = true, copied = false;
         int j = 0, n_seg = 0;
-        while (ok && cursor.next(p.sched, seg)) {
+        bool have = cursor.next(p.sched, seg);
+        for (XSeg seg_next; ok && have; seg = seg_next) {
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
             const bool any = st < u.t1;
+            if (!kKeys && any && !copied) {
+                ok = copy_xy();
+                if (!ok) break;
+            }
             const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
             float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
             if (!kKeys) {
@@ -465,6 +502,17 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
+            // (the next segment's first products run during this one's epilogue)
+            have = cursor.next(p.sched, seg_next);
+            copied = false;
+            if (!kKeys && any && have) {
+                const XBwdUnit un = x_bwd_unit<kKeys>(p, seg_next);
+                if (un.t0 < un.t1) {
+                    ok = copy_xy();
+                    if (!ok) break;
+                    copied = true;
+                }
+            }
             // Each warp writes 32 rows x 64 columns: the key pass's warps those of dk and dv, the query pass's
             // first warps those of dq.
             const int which = kKeys ? piece / (kD / 64) : 0;
@@ -513,7 +561,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             }
             if (any) {
                 tc_fence_before();
-                if (kKeys && lane == 0) tma_store_wait_read();  // (then the owned tiles may be replaced)
+                if (kKeys && lane == 0) tma_store_wait_read();  // (then the next owned tiles may be loaded)
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(smem_u32(&ctl->acc_free));
