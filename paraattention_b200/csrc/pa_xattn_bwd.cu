@@ -8,7 +8,7 @@ namespace {
 
 struct BwdPlan {
     pa::XSched q, k;  // query pass, key pass
-    int grid_q = 0, grid_k = 0, mt = 0, kt = 0, mb = 0, kb = 0;  // 128-row tiles, 64-row blocks
+    int grid_q = 0, grid_k = 0, mt = 0, kt = 0;
     int64_t off_stats = 0, off_part = 0, bytes = 0;
 };
 
@@ -16,12 +16,10 @@ BwdPlan plan(const pa_xattn_args* a) {
     BwdPlan f;
     f.mt = (a->seq_q + 127) / 128;
     f.kt = (a->seq_kv + 127) / 128;
-    f.mb = (a->seq_q + 63) / 64;
-    f.kb = (a->seq_kv + 63) / 64;
     const int sms = sm_count();
-    f.q = xattn_schedule(static_cast<long long>(a->batch) * a->heads * f.mt, f.kb, sms, 8, &f.grid_q);
+    f.q = xattn_schedule(static_cast<long long>(a->batch) * a->heads * f.mt, f.kt, sms, 4, &f.grid_q);
     f.k = xattn_schedule(static_cast<long long>(a->kv_batch) * a->kv_heads * f.kt,
-                         static_cast<long long>(a->batch / a->kv_batch) * (a->heads / a->kv_heads) * f.mb, sms, 8, &f.grid_k);
+                         static_cast<long long>(a->batch / a->kv_batch) * (a->heads / a->kv_heads) * f.mt, sms, 4, &f.grid_k);
     f.off_stats = xattn_mask_layout(a).bytes;
     f.off_part = f.off_stats + int64_t(a->batch) * a->heads * f.mt * 128 * 8;
     // (the passes run one after the other and use the same partial results' space)
@@ -45,16 +43,11 @@ int pass(const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& z, const
 
 template <bool kBF16, int kD>
 int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
-    CUtensorMap mq, mk, mv, mg, mdq, mdk, mdv;  // owned tiles are boxes of 128 rows, streamed blocks of 64, stores of 32
-    CUtensorMap bq, bk, bv, bg;
+    CUtensorMap mq, mk, mv, mg, mdq, mdk, mdv;  // (boxes of 128 rows for loads, 32 for stores)
     int rc = make_map(&mq, a->q, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->q_stride[2], a->q_stride[1], a->q_stride[0], 0, "q");
     if (rc == PA_OK) rc = make_map(&mg, a->dout, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->do_stride[2], a->do_stride[1], a->do_stride[0], 0, "dout");
     if (rc == PA_OK) rc = make_map(&mk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k");
     if (rc == PA_OK) rc = make_map(&mv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v");
-    if (rc == PA_OK) rc = make_map(&bq, a->q, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->q_stride[2], a->q_stride[1], a->q_stride[0], 0, "q", pa::kXStep);
-    if (rc == PA_OK) rc = make_map(&bg, a->dout, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->do_stride[2], a->do_stride[1], a->do_stride[0], 0, "dout", pa::kXStep);
-    if (rc == PA_OK) rc = make_map(&bk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k", pa::kXStep);
-    if (rc == PA_OK) rc = make_map(&bv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v", pa::kXStep);
     if (rc == PA_OK) rc = make_map(&mdq, a->dq, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->dq_stride[2], a->dq_stride[1], a->dq_stride[0], 0, "dq", 32);
     if (rc == PA_OK) rc = make_map(&mdk, a->dk, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dk_stride[2], a->dk_stride[1], a->dk_stride[0], 0, "dk", 32);
     if (rc == PA_OK) rc = make_map(&mdv, a->dv, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dv_stride[2], a->dv_stride[1], a->dv_stride[0], 0, "dv", 32);
@@ -70,7 +63,6 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     p.skv = a->seq_kv;
     p.mt = f.mt;
     p.kt = f.kt;
-    p.mb = f.mb;
     p.scale = a->scale;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.stats = reinterpret_cast<float*>(ws + f.off_stats);
@@ -111,13 +103,13 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     p.g[1] = static_cast<uint16_t*>(a->dv);
     p.g_sb[0] = a->dk_stride[0]; p.g_sh[0] = a->dk_stride[1]; p.g_ss[0] = a->dk_stride[2];
     p.g_sb[1] = a->dv_stride[0]; p.g_sh[1] = a->dv_stride[1]; p.g_ss[1] = a->dv_stride[2];
-    rc = pass<kBF16, kD, true>(mk, mv, bq, bg, mdk, mdv, p, f.grid_k, s);
+    rc = pass<kBF16, kD, true>(mk, mv, mq, mg, mdk, mdv, p, f.grid_k, s);
     if (rc != PA_OK) return rc;
     p.sched = f.q;
     p.g[0] = static_cast<uint16_t*>(a->dq);
     p.g[1] = nullptr;
     p.g_sb[0] = a->dq_stride[0]; p.g_sh[0] = a->dq_stride[1]; p.g_ss[0] = a->dq_stride[2];
-    return pass<kBF16, kD, false>(mq, mg, bk, bv, mdq, mdq, p, f.grid_q, s);
+    return pass<kBF16, kD, false>(mq, mg, mk, mv, mdq, mdq, p, f.grid_q, s);
 }
 
 }  // namespace

@@ -5,26 +5,31 @@
 // the keys for dq; the key pass (kKeys = true) owns tiles of 128 keys and walks the queries (of every
 // head that shares the key head, and of every batch entry that shares the keys) for dk and dv. In
 // both, the owned pair (X, Y) = (q, do) or (k, v) stays on the SM, the other pair (Z, W) = (k, v) or
-// (q, do) streams through a ring in blocks of 64 rows, one block a step, and per step
-//   T1 = X Z^T, T2 = Y W^T                (tensor core, 128 x 64, into TMEM)
+// (q, do) streams through rings in tiles of 128 rows, one tile a step, and per step
+//   T1 = X Z^T, T2 = Y W^T                (tensor core, 128 x 128, into TMEM)
 //   P = 2^(T1 sl - lse'), dS = P (T2 - delta)   (one thread per owned row and 32 columns)
 //   A1 += dS Z  [, A2 += P W in the key pass]   (tensor core, dS and P as TMEM operands)
 // so dS and P never leave TMEM and are never transposed: the key pass computes their transposes
 // to begin with. The price is that S and dP are computed twice (7 products instead of 5); what it
 // buys is no atomics (sums in a fixed order), no fp32 dq traffic, and each gradient written once.
 //
-// Steps alternate between two T buffers, each with its own chain T -> elementwise -> A -> next T: while
-// one is in its elementwise phase the tensor core works on the other. What was measured on the way
-// (16380 queries x 512 keys x 40 heads, cycles per 128 rows, key pass): 8 elementwise warps with 64
-// columns per thread and a ring of two 128-row stages 4600, the tensor core waiting 1600 of them for
-// loads; 16 warps and a ring of four 64-row stages, which are released - and asked for again - half
-// a tile earlier, hide both. The bound then is shared memory: operand fetches of the N = 64 products
-// and the TMA writes are 320 KB per 128 rows of the key pass, 2560 cycles at 128 bytes per cycle.
+// The two products of a step form two chains that hide each other's elementwise phases:
+//   key pass:    A2(j) T1(j+1) | A1(j) T2(j+1) | ...    P(j+1) is made while A1(j), T2(j+1) run,
+//                                                       dS(j+1) while A2(j+1), T1(j+2) run
+//   query pass:  T1(j+1) A1(j) T2(j+1) | ...            P is not an operand: T1(j+1) starts as soon as
+//                                                       T1(j) has been read
+// Measured on the way (16380 queries x 512 keys x 40 heads, cycles per 128 rows, key pass): two chains
+// over half tiles (N = 64 products) 4600 with 8 elementwise warps and a two-stage ring, the tensor
+// core waiting 1600 of them for loads; 4200 with 16 warps and a finer ring, bound by the issue and the
+// operand fetch of the N = 64 products (66 cycles each instead of 32). Whole tiles halve the number of
+// products and their shared-memory traffic per flop: the bound is 2048 cycles of products (64 per
+// 128 x 128 x 16) and as many of shared memory. The query pass holds X and Y in TMEM, where A2 is not
+// needed, and fetches only Z and W from shared memory.
 //
-// Warps 0-15 elementwise (0-7 even steps, 8-15 odd ones), 16 MMA issuer, 17 TMA producer, 18 clears
-// masked rows of K. TMEM columns: T1 [0,128), T2 [128,256) - 64 per buffer -, A1 [256, 256 + D), A2
-// [256 + D, 256 + 2 D); dS overwrites T2, P overwrites T1. CTAs are persistent and the roles run ahead
-// across units (xattn_sm100.cuh divides the work).
+// Warps 0-15 elementwise (32 columns each), 16 MMA issuer, 17 TMA producer, 18 clears masked rows of
+// K. TMEM columns: T1 [0,128), T2 [128,256), A1 [256, 256 + D), A2 [256 + D, 256 + 2 D) or X, Y [384,
+// 512); dS overwrites T2, P overwrites T1. CTAs are persistent and the roles run ahead across units
+// (xattn_sm100.cuh divides the work).
 //
 // What is rounded: P and dS to the tensors' 16-bit type, as operands of a 16-bit product (their
 // relative error, half an ulp, averages out over the sum); everything else is fp32.
@@ -37,19 +42,17 @@ namespace pa {
 constexpr int kXBwdSoftWarps = 16;
 constexpr int kXBwdMmaWarp = 16, kXBwdTmaWarp = 17, kXBwdCleanWarp = 18;
 constexpr int kXBwdThreads = 640;
-constexpr int kXStep = 64;                       // streamed rows per step
-constexpr int kXStages = 4;                      // ring of steps
-constexpr int kXAtomBytes = kXStep * 128;        // 64 rows x 64 elements
-constexpr int kXSlotBytes = 2 * kXAtomBytes;     // a Z or W block (head_dim 64 fills half of it)
+// Z is needed from T1 to A1, W from T2 to A2 or less: three stages of Z and two of W leave every load
+// the time of five products.
+constexpr int kXZStages = 3, kXWStages = 2;
 
 struct XBwdParams {
     int batch, kv_batch, hkv, group, sq, skv;
     int mt, kt;       // 128-row tiles of the queries / of the keys
-    int mb;           // 64-row blocks of the queries
     float scale, scale_log2;
-    uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv (the joining kernel's)
+    uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv (written with TMA, but for joined or empty tiles)
     long long g_sb[2], g_sh[2], g_ss[2];
-    // [B][Hq][2 mt blocks][-lse * log2 e, -delta][64 rows]; rows behind the last query, and rows without
+    // [B][Hq][mt][-lse * log2 e, -delta][128 rows]; rows behind the last query, and rows without
     // any key, have (-inf, 0), which makes their P zero
     const float* stats;
     const unsigned long long* words;
@@ -62,25 +65,22 @@ struct XBwdParams {
 
 struct XBwdCtl {
     uint64_t xy_full, xy_empty;
-    uint64_t xt_full;     // query pass: X and Y are in TMEM (one arrival per warp)
-    uint64_t zw_full[kXStages], zw_empty[kXStages], z_clean[kXStages];
-    uint64_t t_full[2];   // T1 and T2 of a buffer are in TMEM
-    uint64_t p_full[2];   // dS and P of a buffer are in TMEM (one arrival per warp)
-    uint64_t acc_done;    // A1, A2 of a segment are complete
-    uint64_t acc_free;    // the epilogue has read them (one arrival per warp)
+    uint64_t xt_full;               // query pass: X and Y are in TMEM (one arrival per warp)
+    uint64_t z_full[kXZStages], z_empty[kXZStages], z_clean[kXZStages];
+    uint64_t w_full[kXWStages], w_empty[kXWStages];
+    uint64_t t1_full, t2_full;
+    uint64_t p_full;                // key pass: P is in TMEM; query pass: T1 has been read (one arrival per warp)
+    uint64_t ds_full;               // dS is in TMEM (one arrival per warp)
+    uint64_t acc_done;              // A1, A2 of a segment are complete
+    uint64_t acc_free;              // the epilogue has read them (one arrival per warp)
     uint64_t teardown;
     uint32_t tmem_base;
     int abort;
 };
-// Behind the operands: the query pass's staging of dq (8 warps; the key pass stages dk and dv in the
-// memory of the owned tiles, whose segments are long enough for that not to matter), or the key
-// pass's ring of row statistics.
-constexpr int kXBwdExtraBytes = 8 * kXStageBytes;
-// (... and, behind it, a block of zeros for the tiles of keys that no query sees: the owned tiles' memory
-// may hold the next segment's by then)
-constexpr int kXBwdZeroOffset = 4096;
-static_assert(kXStages * kXStep * 8 <= kXBwdZeroOffset && kXBwdZeroOffset + kXStageBytes <= kXBwdExtraBytes, "both fit");
-constexpr int kXBwdSmemBytes = 1024 + 6 * kTileBytes + kXBwdExtraBytes + 512;
+// Operands, the key pass's ring of row statistics, control block. (The dynamic shared memory is declared with the
+// alignment of the swizzle; there is no room for slack.)
+constexpr int kXBwdStatBytes = kXWStages * kTileN * 8;
+constexpr int kXBwdSmemBytes = (2 + kXZStages + kXWStages) * kTileBytes + kXBwdStatBytes + 512;
 static_assert(sizeof(XBwdCtl) <= 512, "control block too large");
 static_assert(kXBwdSmemBytes <= 232448, "shared memory");
 
@@ -90,7 +90,7 @@ struct XBwdUnit {
     int t0, t1;
 };
 struct XBwdStep {
-    int b, head, block;  // streamed 64-row block
+    int b, head, tile;  // streamed tile
 };
 
 template <bool kKeys>
@@ -104,25 +104,25 @@ __device__ __forceinline__ XBwdUnit x_bwd_unit(const XBwdParams& p, const XSeg& 
     u.b = x / heads;
     u.t0 = g.t0;
     u.t1 = g.t1;
-    if (!kKeys && p.extent != nullptr) {  // blocks behind the last key that takes part
-        const int n = (__ldg(p.extent + u.b) + kXStep - 1) / kXStep;
+    if (!kKeys && p.extent != nullptr) {  // key tiles behind the last key that takes part
+        const int n = (__ldg(p.extent + u.b) + kTileN - 1) / kTileN;
         u.t1 = min(u.t1, n);
         u.t0 = min(u.t0, u.t1);
     }
     return u;
 }
-// Key pass: steps run over (batch entries that share the keys, heads of the group, query blocks).
+// Key pass: steps run over (batch entries that share the keys, heads of the group, query tiles).
 template <bool kKeys>
 __device__ __forceinline__ XBwdStep x_bwd_step(const XBwdParams& p, const XBwdUnit& u, int step) {
     XBwdStep s;
     if (!kKeys) {
         s.b = p.kv_batch == 1 ? 0 : u.b;
         s.head = u.head / p.group;
-        s.block = step;
+        s.tile = step;
         return s;
     }
-    const int m = step / p.mb;
-    s.block = step - m * p.mb;
+    const int m = step / p.mt;
+    s.tile = step - m * p.mt;
     const int bb = m / p.group;
     s.head = u.head * p.group + (m - bb * p.group);
     s.b = p.kv_batch == 1 ? bb : u.b;
@@ -133,7 +133,7 @@ __device__ __forceinline__ XBwdStep x_bwd_step(const XBwdParams& p, const XBwdUn
 template <bool kKeys>
 __device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u, int step) {
     if (!kKeys || p.extent == nullptr) return step;
-    const int per_b = p.group * p.mb;
+    const int per_b = p.group * p.mt;
     while (step < u.t1) {
         const int b = p.kv_batch == 1 ? step / per_b : u.b;
         if (u.tile * kTileN < __ldg(p.extent + b)) return step;
@@ -141,6 +141,16 @@ __device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u
         step = (b + 1) * per_b;
     }
     return u.t1;
+}
+// The next segment that has steps, if any.
+template <bool kKeys>
+__device__ __forceinline__ bool x_bwd_more(const XBwdParams& p, XCursor cursor) {
+    XSeg g;
+    while (cursor.next(p.sched, g)) {
+        const XBwdUnit u = x_bwd_unit<kKeys>(p, g);
+        if (x_bwd_live<kKeys>(p, u, u.t0) < u.t1) return true;
+    }
+    return false;
 }
 
 template <bool kBF16, int kD, bool kKeys>
@@ -153,40 +163,46 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     constexpr int kOperandBytes = kAtoms * kHalfBytes;
     constexpr uint32_t kColT1 = 0, kColT2 = 128, kColA1 = 256, kColA2 = 256 + kD;
     constexpr uint32_t kColX = 384, kColY = 448;  // query pass
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw_addr = smem_u32(smem_raw);
-    uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-    const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sZ + kXStages * kXSlotBytes;
-    float* stat = reinterpret_cast<float*>(smem + 6 * kTileBytes);  // [stage][2][64], key pass
-    XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + 6 * kTileBytes + kXBwdExtraBytes);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sZ + kXZStages * kTileBytes;
+    uint8_t* smem_z = smem + 2 * kTileBytes;
+    float* stat = reinterpret_cast<float*>(smem + (2 + kXZStages + kXWStages) * kTileBytes);  // [W stage][2][128], key pass
+    XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + (2 + kXZStages + kXWStages) * kTileBytes + kXBwdStatBytes);
     volatile int* s_abort = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (threadIdx.x == 0) ctl->abort = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+    if (threadIdx.x == 0) {
+        int st = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+        if ((sX & 1023u) != 0) {  // (never seen; the swizzled tiles would not be where the descriptors say)
+            st = PA_DEV_TIMEOUT_PIPE;
+            if (p.status != nullptr) atomicCAS(p.status, 0, st);
+        }
+        ctl->abort = st;
+    }
     __syncthreads();
     if (ctl->abort != 0) return;
     if (threadIdx.x == 0) {
         mbar_init(smem_u32(&ctl->xy_full), 1);
         mbar_init(smem_u32(&ctl->xy_empty), kXBwdSoftWarps);
         mbar_init(smem_u32(&ctl->xt_full), kXBwdSoftWarps);
-        for (int s = 0; s < kXStages; ++s) {
-            mbar_init(smem_u32(&ctl->zw_full[s]), 1);
-            mbar_init(smem_u32(&ctl->zw_empty[s]), 1);
+        for (int s = 0; s < kXZStages; ++s) {
+            mbar_init(smem_u32(&ctl->z_full[s]), 1);
+            mbar_init(smem_u32(&ctl->z_empty[s]), 1);
             mbar_init(smem_u32(&ctl->z_clean[s]), 1);
         }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(smem_u32(&ctl->t_full[s]), 1);
-            mbar_init(smem_u32(&ctl->p_full[s]), kXBwdSoftWarps / 2);
+        for (int s = 0; s < kXWStages; ++s) {
+            mbar_init(smem_u32(&ctl->w_full[s]), 1);
+            // (the key pass's statistics share the stage: the warps that read them arrive too)
+            mbar_init(smem_u32(&ctl->w_empty[s]), kKeys ? 1 + kXBwdSoftWarps : 1);
         }
+        mbar_init(smem_u32(&ctl->t1_full), 1);
+        mbar_init(smem_u32(&ctl->t2_full), 1);
+        mbar_init(smem_u32(&ctl->p_full), kXBwdSoftWarps);
+        mbar_init(smem_u32(&ctl->ds_full), kXBwdSoftWarps);
         mbar_init(smem_u32(&ctl->acc_done), 1);
         mbar_init(smem_u32(&ctl->acc_free), kXBwdSoftWarps);
         mbar_init(smem_u32(&ctl->teardown), 1);
         mbar_init_fence();
-    }
-    if (kKeys) {
-        for (int i = threadIdx.x; i < kXStageBytes / 16; i += kXBwdThreads)
-            reinterpret_cast<uint4*>(smem + 6 * kTileBytes + kXBwdZeroOffset)[i] = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_shared();
     }
     if (warp == kXBwdMmaWarp) {
         tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
@@ -213,13 +229,16 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     if (warp == kXBwdTmaWarp) {
         // =============================== TMA producer ======================================
         if (lane == 0) {
+            auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                return mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+            };
             bool ok = true;
             int j = 0, n_seg = 0;
             while (ok && cursor.next(p.sched, seg)) {
                 const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
                 int st = x_bwd_live<kKeys>(p, u, u.t0);
                 if (st >= u.t1) continue;
-                if (n_seg > 0) ok = mbar_wait(smem_u32(&ctl->xy_empty), (n_seg - 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                if (n_seg > 0) ok = wait(&ctl->xy_empty, (n_seg - 1) & 1);
                 if (!ok) break;
                 const uint32_t bx = smem_u32(&ctl->xy_full);
                 mbar_expect_tx(bx, 2 * kOperandBytes);
@@ -230,23 +249,27 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 }
                 for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
                     const XBwdStep s = x_bwd_step<kKeys>(p, u, st);
-                    const int sg = j % kXStages;
-                    const uint32_t bz = smem_u32(&ctl->zw_full[sg]);
-                    if (j >= kXStages)
-                        ok = mbar_wait(smem_u32(&ctl->zw_empty[sg]), ((j / kXStages) & 1) ^ 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
+                    const int zs = j % kXZStages, ws = j % kXWStages;
+                    if (j >= kXZStages) ok = wait(&ctl->z_empty[zs], ((j / kXZStages) & 1) ^ 1);
                     if (!ok) break;
-                    mbar_expect_tx(bz, 2 * kAtoms * kXAtomBytes + (kKeys ? kXStep * 8 : 0));
+                    const uint32_t bz = smem_u32(&ctl->z_full[zs]);
+                    mbar_expect_tx(bz, kOperandBytes);
 #pragma unroll
-                    for (int h = 0; h < kAtoms; ++h) {
-                        tma_load_5d(sZ + sg * kXSlotBytes + h * kXAtomBytes, &tm_z, bz, h * 64, s.block * kXStep, s.head, s.b, 0);
-                        tma_load_5d(sW + sg * kXSlotBytes + h * kXAtomBytes, &tm_w, bz, h * 64, s.block * kXStep, s.head, s.b, 0);
-                    }
+                    for (int h = 0; h < kAtoms; ++h)
+                        tma_load_5d(sZ + zs * kTileBytes + h * kHalfBytes, &tm_z, bz, h * 64, s.tile * kTileN, s.head, s.b, 0);
+                    if (j >= kXWStages) ok = wait(&ctl->w_empty[ws], ((j / kXWStages) & 1) ^ 1);
+                    if (!ok) break;
+                    const uint32_t bw = smem_u32(&ctl->w_full[ws]);
+                    mbar_expect_tx(bw, kOperandBytes + (kKeys ? kTileN * 8 : 0));
+#pragma unroll
+                    for (int h = 0; h < kAtoms; ++h)
+                        tma_load_5d(sW + ws * kTileBytes + h * kHalfBytes, &tm_w, bw, h * 64, s.tile * kTileN, s.head, s.b, 0);
                     if (kKeys) {
-                        const float* src = p.stats + ((static_cast<long long>(s.b) * p.hkv * p.group + s.head) * (2 * p.mt) + s.block) * (2 * kXStep);
+                        const float* src = p.stats + ((static_cast<long long>(s.b) * p.hkv * p.group + s.head) * p.mt + s.tile) * (2 * kTileN);
                         asm volatile(
                             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                smem_u32(stat + sg * 2 * kXStep)),
-                            "l"(src), "r"(kXStep * 8), "r"(bz)
+                                smem_u32(stat + ws * 2 * kTileN)),
+                            "l"(src), "r"(kTileN * 8), "r"(bw)
                             : "memory");
                     }
                 }
@@ -257,97 +280,96 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 volatile int* no_abort = &none;
                 if (n_seg > 0) mbar_wait(smem_u32(&ctl->xy_full), (n_seg - 1) & 1, no_abort, nullptr, 10000000ull, 0);
                 mbar_wait(smem_u32(&ctl->xy_full), n_seg & 1, no_abort, nullptr, 10000000ull, 0);
-                for (int jj = (j > kXStages ? j - kXStages : 0); jj <= j; ++jj)
-                    mbar_wait(smem_u32(&ctl->zw_full[jj % kXStages]), (jj / kXStages) & 1, no_abort, nullptr, 10000000ull, 0);
+                for (int jj = (j > kXZStages ? j - kXZStages : 0); jj <= j; ++jj) {
+                    mbar_wait(smem_u32(&ctl->z_full[jj % kXZStages]), (jj / kXZStages) & 1, no_abort, nullptr, 10000000ull, 0);
+                    mbar_wait(smem_u32(&ctl->w_full[jj % kXWStages]), (jj / kXWStages) & 1, no_abort, nullptr, 10000000ull, 0);
+                }
             }
         }
     } else if (warp == kXBwdMmaWarp) {
         // =============================== MMA issuer ========================================
-        constexpr uint32_t idesc_t = make_idesc_f16(kBF16, false, kTileM, 64);
+        constexpr uint32_t idesc_t = make_idesc_f16(kBF16, false, kTileM, kTileN);
         constexpr uint32_t idesc_a = make_idesc_f16(kBF16, true, kTileM, kD);
         const uint32_t leader = elect_one() ? 1u : 0u;
         // K-major descriptors (T1, T2) and MN-major descriptors (the same tiles as B operands of A1, A2)
-        const uint64_t dk0 = smem_desc_sw128(sX, 16, 1024), dm0 = smem_desc_sw128(sZ, kXAtomBytes, 1024);
+        const uint64_t dk0 = smem_desc_sw128(sX, 16, 1024), dm0 = smem_desc_sw128(sZ, kHalfBytes, 1024);
         const uint32_t hi_k = static_cast<uint32_t>(dk0 >> 32), hi_m = static_cast<uint32_t>(dm0 >> 32);
         const uint32_t lo_x = static_cast<uint32_t>(dk0), lo_y = lo_x + (kTileBytes >> 4);
-        const uint32_t lo_z = static_cast<uint32_t>(smem_desc_sw128(sZ, 16, 1024)), lo_w = lo_z + (kXStages * kXSlotBytes >> 4);
-        const uint32_t lo_zm = static_cast<uint32_t>(dm0), lo_wm = lo_zm + (kXStages * kXSlotBytes >> 4);
-        // T of the step in ring slot sg into buffer t
-        auto issue_t = [&](int sg, int t) {
-            const uint32_t zo = (sg * kXSlotBytes) >> 4;
+        const uint32_t lo_z = static_cast<uint32_t>(smem_desc_sw128(sZ, 16, 1024)), lo_w = lo_z + (kXZStages * kTileBytes >> 4);
+        const uint32_t lo_zm = static_cast<uint32_t>(dm0), lo_wm = lo_zm + (kXZStages * kTileBytes >> 4);
+        auto issue_t = [&](uint32_t lo_own, uint32_t col_own, uint32_t lo_b, uint32_t col, uint64_t* full) {
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
-                const uint32_t ao = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4, bo = ((ks >> 2) * kXAtomBytes + (ks & 3) * 32) >> 4;
-                if (kKeys) tc_mma_ss_elect(tmem + kColT1 + t * 64, lo_x + ao, hi_k, lo_z + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
-                else tc_mma_ts_elect(tmem + kColT1 + t * 64, tmem + kColX + ks * 8, lo_z + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+                if (kKeys) tc_mma_ss_elect(tmem + col, lo_own + off, hi_k, lo_b + off, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
+                else tc_mma_ts_elect(tmem + col, tmem + col_own + ks * 8, lo_b + off, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
             }
-#pragma unroll
-            for (int ks = 0; ks < kD / 16; ++ks) {
-                const uint32_t ao = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4, bo = ((ks >> 2) * kXAtomBytes + (ks & 3) * 32) >> 4;
-                if (kKeys) tc_mma_ss_elect(tmem + kColT2 + t * 64, lo_y + ao, hi_k, lo_w + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
-                else tc_mma_ts_elect(tmem + kColT2 + t * 64, tmem + kColY + ks * 8, lo_w + zo + bo, hi_k, idesc_t, ks > 0 ? 1u : 0u, leader);
-            }
-            tc_commit_elect(smem_u32(&ctl->t_full[t]), leader);
+            tc_commit_elect(smem_u32(full), leader);
         };
-        // (16 streamed rows a k-step; their dS / P are 8 packed columns, 32 columns of T packed into 16)
-        auto issue_a = [&](int sg, int t, bool acc) {
-            const uint32_t so = (sg * kXSlotBytes) >> 4;
+        auto issue_t1 = [&](int j) { issue_t(lo_x, kColX, lo_z + ((j % kXZStages) * kTileBytes >> 4), kColT1, &ctl->t1_full); };
+        auto issue_t2 = [&](int j) {
+            issue_t(lo_y, kColY, lo_w + ((j % kXWStages) * kTileBytes >> 4), kColT2, &ctl->t2_full);
+            if (!kKeys) tc_commit_elect(smem_u32(&ctl->w_empty[j % kXWStages]), leader);
+        };
+        // 16 streamed rows a k-step; their dS / P are 8 packed columns (32 columns of T are packed into 16)
+        auto issue_a = [&](uint32_t col_a, uint32_t col_t, uint32_t lo_b, bool acc) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-                tc_mma_ts_elect(tmem + kColA1, tmem + kColT2 + t * 64 + (ks >> 1) * 32 + (ks & 1) * 8, lo_zm + so + ((ks * 16 * 128) >> 4),
-                                hi_m, idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
-            if (kKeys) {
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    tc_mma_ts_elect(tmem + kColA2, tmem + kColT1 + t * 64 + (ks >> 1) * 32 + (ks & 1) * 8,
-                                    lo_wm + so + ((ks * 16 * 128) >> 4), hi_m, idesc_a, (acc || ks > 0) ? 1u : 0u, leader);
-            }
+            for (int ks = 0; ks < 8; ++ks)
+                tc_mma_ts_elect(tmem + col_a, tmem + col_t + (ks >> 1) * 32 + (ks & 1) * 8, lo_b + ((ks * 16 * 128) >> 4), hi_m, idesc_a,
+                                (acc || ks > 0) ? 1u : 0u, leader);
         };
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-            const bool r = mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
-            return __all_sync(0xffffffffu, r);
+            const bool r = __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE));
+            tc_fence_after();
+            return r;
         };
-        auto wait_zw = [&](int j) -> bool {
-            return wait(clean ? &ctl->z_clean[j % kXStages] : &ctl->zw_full[j % kXStages], (j / kXStages) & 1);
+        auto wait_z = [&](int j) -> bool {
+            return wait(clean ? &ctl->z_clean[j % kXZStages] : &ctl->z_full[j % kXZStages], (j / kXZStages) & 1);
         };
+        auto wait_w = [&](int j) -> bool { return wait(&ctl->w_full[j % kXWStages], (j / kXWStages) & 1); };
         bool ok = true, issued = false;
         int j = 0, n_seg = 0;  // steps, segments with steps
         while (ok && cursor.next(p.sched, seg)) {
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
             if (st >= u.t1) continue;
-            // T runs two steps ahead of A
-            int ahead = x_bwd_live<kKeys>(p, u, st + 1);
-            ok = wait(kKeys ? &ctl->xy_full : &ctl->xt_full, n_seg & 1) && wait_zw(j);
+            ok = wait(kKeys ? &ctl->xy_full : &ctl->xt_full, n_seg & 1) && wait_z(j);
             if (!ok) break;
-            tc_fence_after();
             issued = true;
-            issue_t(j % kXStages, j & 1);
-            bool two = ahead < u.t1;
-            if (two) {
-                ok = wait_zw(j + 1);
-                if (!ok) break;
-                tc_fence_after();
-                issue_t((j + 1) % kXStages, (j + 1) & 1);
-                ahead = x_bwd_live<kKeys>(p, u, ahead + 1);
-            }
-            int left = two ? 2 : 1;  // steps whose T is issued and whose A is not
-            for (bool first = true; left > 0; first = false, ++j) {
-                ok = wait(&ctl->p_full[j & 1], (j >> 1) & 1);
+            issue_t1(j);
+            ok = wait_w(j);
+            if (!ok) break;
+            issue_t2(j);
+            for (bool first = true; st < u.t1; first = false, ++j) {
+                st = x_bwd_live<kKeys>(p, u, st + 1);
+                const bool more = st < u.t1;
                 // (the accumulators of the segment before have been read by the epilogue)
-                if (ok && first && n_seg > 0) ok = wait(&ctl->acc_free, (n_seg - 1) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                issue_a(j % kXStages, j & 1, !first);
-                tc_commit_elect(smem_u32(&ctl->zw_empty[j % kXStages]), leader);
-                --left;
-                if (ahead < u.t1) {
-                    ok = wait_zw(j + 2);
+                if (kKeys) {
+                    ok = wait(&ctl->p_full, j & 1) && (!first || n_seg == 0 || wait(&ctl->acc_free, (n_seg - 1) & 1));
                     if (!ok) break;
-                    tc_fence_after();
-                    issue_t((j + 2) % kXStages, j & 1);
-                    ++left;
-                    ahead = x_bwd_live<kKeys>(p, u, ahead + 1);
+                    issue_a(kColA2, kColT1, lo_wm + ((j % kXWStages) * kTileBytes >> 4), !first);
+                    tc_commit_elect(smem_u32(&ctl->w_empty[j % kXWStages]), leader);
+                    if (more) {
+                        ok = wait_z(j + 1);
+                        if (!ok) break;
+                        issue_t1(j + 1);
+                    }
+                    ok = wait(&ctl->ds_full, j & 1);
+                } else {
+                    if (more) {
+                        ok = wait_z(j + 1) && wait(&ctl->p_full, j & 1);
+                        if (!ok) break;
+                        issue_t1(j + 1);
+                    }
+                    ok = wait(&ctl->ds_full, j & 1) && (!first || n_seg == 0 || wait(&ctl->acc_free, (n_seg - 1) & 1));
+                }
+                if (!ok) break;
+                issue_a(kColA1, kColT2, lo_zm + ((j % kXZStages) * kTileBytes >> 4), !first);
+                tc_commit_elect(smem_u32(&ctl->z_empty[j % kXZStages]), leader);
+                if (more) {
+                    ok = wait_w(j + 1);
+                    if (!ok) break;
+                    issue_t2(j + 1);
                 }
             }
             if (!ok) break;
@@ -368,34 +390,41 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             const unsigned long long* row = p.words + static_cast<long long>(u.b) * n_words;
             for (int t = u.t0; t < u.t1; ++t, ++j) {
-                const int sg = j % kXStages;
-                const unsigned long long word = x_key_word(row, p.skv, t);
-                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->zw_full[sg]), (j / kXStages) & 1, s_abort, p.status, limit,
+                const int zs = j % kXZStages;
+                const unsigned long long w0 = x_key_word(row, p.skv, 2 * t), w1 = x_key_word(row, p.skv, 2 * t + 1);
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->z_full[zs]), (j / kXZStages) & 1, s_abort, p.status, limit,
                                                        PA_DEV_TIMEOUT_PIPE));
                 if (!ok) break;
-                if (word != ~0ull) {
-                    x_zero_rows<kD>(smem + 2 * kTileBytes + sg * kXSlotBytes, kXAtomBytes, word, lane);
+                if ((w0 & w1) != ~0ull) {
+                    x_zero_rows<kD>(smem_z + zs * kTileBytes, kHalfBytes, w0, lane);
+                    x_zero_rows<kD>(smem_z + zs * kTileBytes + 64 * 128, kHalfBytes, w1, lane);
                     fence_proxy_async_shared();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->z_clean[sg]));
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->z_clean[zs]));
             }
         }
     } else if (warp < kXBwdSoftWarps) {
         // =============================== elementwise + epilogue ============================
-        const int quarter = warp & 3, piece = warp >> 2, buf = piece >> 1;  // my lanes; my 32 columns; their T buffer
+        const int quarter = warp & 3, piece = warp >> 2;  // my lanes; my 32 columns
         const int row_in_tile = quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t t1 = tmem + lane_base + kColT1 + piece * 32, t2 = tmem + lane_base + kColT2 + piece * 32;
         // (dS and P of my 32 columns are packed into the first 16 of them: no other warp reads or writes there)
         const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+        // (a vote: a wait that gives up in some lanes only must not split the warp)
+        auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+            return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE));
+        };
+        auto arrive = [&](uint64_t* bar) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(bar));
+        };
         // Query pass: brings a segment's X and Y from shared memory to TMEM once its predecessor's products
-        // are done (false: a wait gave up). D / 8 16-byte chunks per row, four of them per warp.
+        // are done. D / 8 16-byte chunks per row, four of them per warp.
         int n_copied = 0;
         auto copy_xy = [&]() -> bool {
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->xy_full), n_copied & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE)))
-                return false;
-            ++n_copied;
+            if (!wait(&ctl->xy_full, n_copied & 1)) return false;
             if (piece * 4 < kD / 8) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
@@ -411,38 +440,33 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 tc_wait_st();
             }
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(smem_u32(&ctl->xt_full));
-                mbar_arrive(smem_u32(&ctl->xy_empty));
-            }
-            return true;
+            arrive(&ctl->xt_full);
+            // (the epilogue that follows reuses the memory: all warps must have read it)
+            return wait(&ctl->xt_full, n_copied++ & 1);
         };
-        bool ok = true, copied = false;
+        bool ok = true;
         int j = 0, n_seg = 0;
-        bool have = cursor.next(p.sched, seg);
-        for (XSeg seg_next; ok && have; seg = seg_next) {
+        while (ok && cursor.next(p.sched, seg)) {
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
             const bool any = st < u.t1;
-            if (!kKeys && any && !copied) {
+            if (!kKeys && any && n_seg == 0) {
                 ok = copy_xy();
                 if (!ok) break;
+                arrive(&ctl->xy_empty);
             }
             const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
             float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
             if (!kKeys) {
-                const float* r = p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * (2 * p.mt) + (row >> 6)) * (2 * kXStep) + (row & 63);
+                const float* r = p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt + u.tile) * (2 * kTileN) + row_in_tile;
                 neg.x = neg.y = __ldg(r);
-                dl.x = dl.y = __ldg(r + kXStep);
+                dl.x = dl.y = __ldg(r + kTileN);
             }
             for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
-                if ((j & 1) != buf) continue;
                 uint32_t live = 0xffffffffu;  // query pass: my columns' keys; key pass: all or nothing
                 if (!kKeys) {
-                    live = static_cast<uint32_t>(
-                        x_key_word(p.words != nullptr ? p.words + static_cast<long long>(u.b) * n_words : nullptr, p.skv, st) >>
-                        ((piece & 1) * 32));
+                    live = static_cast<uint32_t>(x_key_word(p.words != nullptr ? p.words + static_cast<long long>(u.b) * n_words : nullptr,
+                                                            p.skv, 2 * st + (piece >> 1)) >> ((piece & 1) * 32));
                 } else if (p.words != nullptr) {
                     const int b = x_bwd_step<kKeys>(p, u, st).b;
                     if (row >= p.skv || ((__ldg(p.words + static_cast<long long>(b) * n_words + (row >> 6)) >> (row & 63)) & 1ull) == 0) live = 0u;
@@ -450,122 +474,156 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                     live = 0u;
                 }
                 const bool plain = __all_sync(0xffffffffu, live == 0xffffffffu);
-                if (kKeys)  // (the step's statistics are in shared memory: already true when t_full is)
-                    ok = mbar_wait(smem_u32(&ctl->zw_full[j % kXStages]), (j / kXStages) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
-                ok = mbar_wait(smem_u32(&ctl->t_full[buf]), (j >> 1) & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE) && ok;
-                ok = __all_sync(0xffffffffu, ok);
+                // (key pass: the step's statistics come with W)
+                const float4* cl = reinterpret_cast<const float4*>(stat + (j % kXWStages) * 2 * kTileN + piece * 32);
+                if (kKeys) ok = wait(&ctl->w_full[j % kXWStages], (j / kXWStages) & 1);
+                ok = ok && wait(&ctl->t1_full, j & 1);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t a[32], d[32];
+                uint32_t a[32];
                 tmem_ld32(t1, a);
-                tmem_ld32(t2, d);
                 tc_wait_ld();
                 tmem_ld_fence(a);
-                tmem_ld_fence(d);
-                const float4* cl = reinterpret_cast<const float4*>(stat + (j % kXStages) * 2 * kXStep + (piece & 1) * 32);
-                uint32_t pp[16], ds[16];
+                if (!kKeys) {
+                    tc_fence_before();
+                    arrive(&ctl->p_full);
+                }
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
-                    float2 ng[2] = {neg, neg}, dt[2] = {dl, dl};
+                    float2 ng[2] = {neg, neg};
                     if (kKeys) {
-                        const float4 l4 = cl[i >> 2], d4 = cl[(i >> 2) + kXStep / 4];
+                        const float4 l4 = cl[i >> 2];
                         ng[0] = make_float2(l4.x, l4.y);
                         ng[1] = make_float2(l4.z, l4.w);
+                    }
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int c = i + 2 * y;
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), sl2, ng[y]);
+                        float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
+                        if (!plain) {
+                            if (((live >> c) & 1u) == 0) e0 = 0.f;
+                            if (((live >> (c + 1)) & 1u) == 0) e1 = 0.f;
+                        }
+                        a[c] = __float_as_uint(e0);
+                        a[c + 1] = __float_as_uint(e1);
+                    }
+                }
+                if (kKeys) {
+                    uint32_t pp[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        pp[i] = kBF16 ? pack_bf16x2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]))
+                                      : pack_f16x2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+                    tmem_st16(t1, pp);
+                    tc_wait_st();
+                    tc_fence_before();
+                    arrive(&ctl->p_full);
+                }
+                ok = wait(&ctl->t2_full, j & 1);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t d[32], ds[16];
+                tmem_ld32(t2, d);
+                tc_wait_ld();
+                tmem_ld_fence(d);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float2 dt[2] = {dl, dl};
+                    if (kKeys) {
+                        const float4 d4 = cl[(i >> 2) + kTileN / 4];
                         dt[0] = make_float2(d4.x, d4.y);
                         dt[1] = make_float2(d4.z, d4.w);
                     }
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         const int c = i + 2 * y;
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), sl2, ng[y]);
-                        float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                        float2 s = __fmul2_rn(e, __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dt[y]));
-                        if (!plain) {
-                            if (((live >> c) & 1u) == 0) e.x = s.x = 0.f;
-                            if (((live >> (c + 1)) & 1u) == 0) e.y = s.y = 0.f;
+                        float2 s = __fmul2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])),
+                                              __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dt[y]));
+                        if (!plain) {  // (T2 of a masked key may be anything)
+                            if (((live >> c) & 1u) == 0) s.x = 0.f;
+                            if (((live >> (c + 1)) & 1u) == 0) s.y = 0.f;
                         }
-                        if (kKeys) pp[c >> 1] = kBF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
                         ds[c >> 1] = kBF16 ? pack_bf16x2(s.x, s.y) : pack_f16x2(s.x, s.y);
                     }
                 }
                 tmem_st16(t2, ds);
-                if (kKeys) tmem_st16(t1, pp);
                 tc_wait_st();
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl->p_full[buf]));
+                arrive(&ctl->ds_full);
+                if (kKeys && lane == 0) mbar_arrive(smem_u32(&ctl->w_empty[j % kXWStages]));
             }
-            if (any && ok) {
-                ok = mbar_wait(smem_u32(&ctl->acc_done), n_seg & 1, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
-                ++n_seg;
-            }
-            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            tc_fence_after();
-            // (the next segment's first products run during this one's epilogue)
-            have = cursor.next(p.sched, seg_next);
-            copied = false;
-            if (!kKeys && any && have) {
-                const XBwdUnit un = x_bwd_unit<kKeys>(p, seg_next);
-                if (un.t0 < un.t1) {
+            bool copied = false;
+            if (any) {
+                ok = wait(&ctl->acc_done, n_seg & 1);
+                if (!ok) break;
+                tc_fence_after();
+                ++n_seg;
+                // (the next segment's first products run during this one's epilogue)
+                if (!kKeys && x_bwd_more<kKeys>(p, cursor)) {
                     ok = copy_xy();
                     if (!ok) break;
                     copied = true;
                 }
             }
             // Each warp writes 32 rows x 64 columns: the key pass's warps those of dk and dv, the query pass's
-            // first warps those of dq.
+            // first warps those of dq; staged where the owned tiles were, which are no longer needed.
             const int which = kKeys ? piece / (kD / 64) : 0;
             const int cb = kKeys ? piece % (kD / 64) : piece;  // 64-column block
-            const bool mine = which < 2 && cb < kD / 64;
-            if (kKeys && !any && mine && seg.slot < 0) {
-                const int row_w = u.tile * kTileM + quarter * 32;
-                if (lane == 0 && row_w < p.skv)
-                    tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(smem + 6 * kTileBytes + kXBwdZeroOffset), cb * 64, row_w, u.head, u.b, 0);
-            } else if (mine) {
+            if (which < 2 && cb < kD / 64) {
                 const uint32_t ta = tmem + lane_base + (which ? kColA2 : kColA1) + cb * 64;
                 const int row_w = u.tile * kTileM + quarter * 32;
-                uint8_t* stage = kKeys ? smem + warp * kXStageBytes : smem + 6 * kTileBytes + warp * kXStageBytes;
-                if (seg.slot < 0) {
-                    if (lane == 0) tma_store_wait_read();  // (the staging memory is free again)
-                    __syncwarp();
-                }
+                uint8_t* stage = smem + warp * kXStageBytes;
+                const int rows = kKeys ? p.skv : p.sq;
+                if (!any && seg.slot < 0) {
+                    // nothing to add up: zeros, stored directly (the memory may hold the next owned tiles)
+                    if (row < rows) {
+                        uint4* dst = reinterpret_cast<uint4*>(p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]) + cb * 64);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t o[32];
-                    tmem_ld32(ta + b * 32, o);
-                    tc_wait_ld();
-                    tmem_ld_fence(o);
-                    if (!any) {
+                        for (int x = 0; x < 8; ++x) dst[x] = make_uint4(0, 0, 0, 0);
+                    }
+                } else {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = 0u;
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t o[32];
+                        tmem_ld32(ta + b * 32, o);
+                        tc_wait_ld();
+                        tmem_ld_fence(o);
+                        if (!any) {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) o[x] = 0u;
+                        }
+                        if (seg.slot < 0) {
+                            x_stage32<kBF16>(stage, lane, b, o, which ? 1.0f : p.scale);
+                        } else {
+                            float4* part = reinterpret_cast<float4*>(p.part) +
+                                           ((static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) + cb * 16 + b * 8) * kTileM + row_in_tile;
+#pragma unroll
+                            for (int v4 = 0; v4 < 8; ++v4)
+                                __stcg(part + v4 * kTileM,
+                                       make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
+                                                   __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
+                        }
                     }
                     if (seg.slot < 0) {
-                        x_stage32<kBF16>(stage, lane, b, o, which ? 1.0f : p.scale);
-                    } else {
-                        float4* part = reinterpret_cast<float4*>(p.part) +
-                                       ((static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) + cb * 16 + b * 8) * kTileM + row_in_tile;
-#pragma unroll
-                        for (int v4 = 0; v4 < 8; ++v4)
-                            __stcg(part + v4 * kTileM,
-                                   make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
-                                               __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
+                        fence_proxy_async_shared();
+                        __syncwarp();
+                        if (lane == 0 && row_w < rows)
+                            tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(stage), cb * 64, row_w, u.head, u.b, 0);
                     }
-                }
-                if (seg.slot < 0) {
-                    fence_proxy_async_shared();
-                    __syncwarp();
-                    if (lane == 0 && row_w < (kKeys ? p.skv : p.sq))
-                        tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(stage), cb * 64, row_w, u.head, u.b, 0);
                 }
             }
             if (any) {
                 tc_fence_before();
-                if (kKeys && lane == 0) tma_store_wait_read();  // (then the next owned tiles may be loaded)
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&ctl->acc_free));
-                    if (kKeys) mbar_arrive(smem_u32(&ctl->xy_empty));
+                arrive(&ctl->acc_free);
+                // the owned tiles' memory may be loaded again: key pass, the next ones; query pass, those behind
+                // the ones already copied
+                if (kKeys || copied) {
+                    if (lane == 0) {
+                        tma_store_wait_read();
+                        mbar_arrive(smem_u32(&ctl->xy_empty));
+                    }
                 }
             }
         }
@@ -620,13 +678,13 @@ xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, int grid) {
     }
 }
 
-// stats[b][h][64-row block][0 / 1][64] = -lse * log2 e and -sum_d do * out of the query rows; (-inf, 0) for rows without
+// stats[b][h][tile][0 / 1][128] = -lse * log2 e and -sum_d do * out of the query rows; (-inf, 0) for rows without
 // any key and behind the last one. HBM-bound: one pass over do and out, 16 bytes per lane.
 struct XStatParams {
     const uint16_t *o, *g;  // out, do
     long long o_s[3], g_s[3];
     const float* lse;  // [B][Hq][Sq]
-    float* stats;      // [B][Hq][padded / 64][2][64]
+    float* stats;      // [B][Hq][padded / 128][2][128]
     int batch, heads, sq, padded;
 };
 constexpr int kXStatThreads = 256;
@@ -665,9 +723,9 @@ xattn_stat_kernel(const __grid_constant__ XStatParams p) {
                 const float l = __ldg(p.lse + (static_cast<long long>(b) * p.heads + h) * p.sq + s);
                 if (l != -INFINITY) r = make_float2(l * -1.4426950408889634f, -dot);
             }
-            float* dst = p.stats + (static_cast<long long>(b) * p.heads + h) * p.padded * 2 + (s / kXStep) * (2 * kXStep) + s % kXStep;
+            float* dst = p.stats + (static_cast<long long>(b) * p.heads + h) * p.padded * 2 + (s / kTileN) * (2 * kTileN) + s % kTileN;
             dst[0] = r.x;
-            dst[kXStep] = r.y;
+            dst[kTileN] = r.y;
         }
     }
 }
