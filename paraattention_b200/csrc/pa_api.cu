@@ -69,9 +69,9 @@ EncodeTiledFn get_encode_fn() {
 }  // namespace
 
 // 5-D map over [chunk][batch][head][row][head_dim] with element strides (head_dim stride 1); the box is
-// 64 elements x box_rows rows with the 128-byte swizzle the MMA descriptors expect.
+// 64 elements x 128 rows with the 128-byte swizzle the MMA descriptors expect, unless asked otherwise.
 int make_map(CUtensorMap* map, const void* base, int dtype, int head_dim, int rows, int heads, int batch, int chunks,
-             int64_t s_row, int64_t s_head, int64_t s_batch, int64_t s_chunk, const char* what, int box_rows) {
+             int64_t s_row, int64_t s_head, int64_t s_batch, int64_t s_chunk, const char* what, int box_rows, int box_cols) {
     EncodeTiledFn enc = get_encode_fn();
     if (enc == nullptr) return fail(PA_ECUDA, "cuTensorMapEncodeTiled is not available from this driver");
     if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0)
@@ -88,12 +88,13 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int head_dim, int ro
         if (static_cast<uint64_t>(s) * 2 >= (1ull << 40)) return fail(PA_EINVAL, "%s: stride %d too large", what, i);
         strides[i] = static_cast<cuuint64_t>(s) * 2;
     }
-    cuuint32_t box[5] = {64, static_cast<cuuint32_t>(box_rows), 1, 1, 1};
+    cuuint32_t box[5] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1, 1, 1};
     cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     CUtensorMapDataType dt = dtype == PA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     auto encode = [&] {
         return enc(map, dt, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
     CUresult r = encode();
     if (r == CUDA_ERROR_INVALID_CONTEXT) {

@@ -43,14 +43,14 @@ int pass(const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& z, const
 
 template <bool kBF16, int kD>
 int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
-    CUtensorMap mq, mk, mv, mg, mdq, mdk, mdv;  // (boxes of 128 rows for loads, 32 for stores)
+    CUtensorMap mq, mk, mv, mg, mdq, mdk, mdv;  // (boxes of 128 x 64 for loads, 32 x 32 for stores)
     int rc = make_map(&mq, a->q, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->q_stride[2], a->q_stride[1], a->q_stride[0], 0, "q");
     if (rc == PA_OK) rc = make_map(&mg, a->dout, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->do_stride[2], a->do_stride[1], a->do_stride[0], 0, "dout");
     if (rc == PA_OK) rc = make_map(&mk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k");
     if (rc == PA_OK) rc = make_map(&mv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v");
-    if (rc == PA_OK) rc = make_map(&mdq, a->dq, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->dq_stride[2], a->dq_stride[1], a->dq_stride[0], 0, "dq", 32);
-    if (rc == PA_OK) rc = make_map(&mdk, a->dk, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dk_stride[2], a->dk_stride[1], a->dk_stride[0], 0, "dk", 32);
-    if (rc == PA_OK) rc = make_map(&mdv, a->dv, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dv_stride[2], a->dv_stride[1], a->dv_stride[0], 0, "dv", 32);
+    if (rc == PA_OK) rc = make_map(&mdq, a->dq, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->dq_stride[2], a->dq_stride[1], a->dq_stride[0], 0, "dq", 32, 32);
+    if (rc == PA_OK) rc = make_map(&mdk, a->dk, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dk_stride[2], a->dk_stride[1], a->dk_stride[0], 0, "dk", 32, 32);
+    if (rc == PA_OK) rc = make_map(&mdv, a->dv, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dv_stride[2], a->dv_stride[1], a->dv_stride[0], 0, "dv", 32, 32);
     if (rc != PA_OK) return rc;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     pa::XBwdParams p;

@@ -88,7 +88,7 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     int rc = make_map(&mq, a->q, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->q_stride[2], a->q_stride[1], a->q_stride[0], 0, "q");
     if (rc == PA_OK) rc = make_map(&mk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k");
     if (rc == PA_OK) rc = make_map(&mv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v");
-    if (rc == PA_OK) rc = make_map(&mo, a->out, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->o_stride[2], a->o_stride[1], a->o_stride[0], 0, "out", 32);
+    if (rc == PA_OK) rc = make_map(&mo, a->out, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->o_stride[2], a->o_stride[1], a->o_stride[0], 0, "out", 32, 32);
     if (rc != PA_OK) return rc;
     pa::XFwdParams p;
     memset(&p, 0, sizeof(p));

@@ -412,7 +412,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         const uint32_t t1 = tmem + lane_base + kColT1 + piece * 32, t2 = tmem + lane_base + kColT2 + piece * 32;
         // (dS and P of my 32 columns are packed into the first 16 of them: no other warp reads or writes there)
         const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-        // (a vote: a wait that gives up in some lanes only must not split the warp)
+        // (a vote: it brings the lanes together again, and a wait that gives up in some of them must not split the warp)
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
             return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE));
         };
@@ -441,8 +441,20 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             }
             tc_fence_before();
             arrive(&ctl->xt_full);
-            // (the epilogue that follows reuses the memory: all warps must have read it)
-            return wait(&ctl->xt_full, n_copied++ & 1);
+            ++n_copied;
+            return true;
+        };
+        auto row_stats = [&](const XBwdUnit& u) -> const float* {
+            return p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt + u.tile) * (2 * kTileN) + row_in_tile;
+        };
+        // Tells the producer that the owned tiles' memory may be loaded again (the stores staged there have been read).
+        bool owe_release = false;
+        auto release_xy = [&]() {
+            if (owe_release && lane == 0) {
+                tma_store_wait_read();
+                mbar_arrive(smem_u32(&ctl->xy_empty));
+            }
+            owe_release = false;
         };
         bool ok = true;
         int j = 0, n_seg = 0;
@@ -453,18 +465,20 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             if (!kKeys && any && n_seg == 0) {
                 ok = copy_xy();
                 if (!ok) break;
-                arrive(&ctl->xy_empty);
+                owe_release = true;
             }
             const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
             float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
             if (!kKeys) {
-                const float* r = p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt + u.tile) * (2 * kTileN) + row_in_tile;
+                const float* r = row_stats(u);
                 neg.x = neg.y = __ldg(r);
                 dl.x = dl.y = __ldg(r + kTileN);
             }
-            for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
+            const bool whole = p.words == nullptr && (!kKeys || (u.tile + 1) * kTileM <= p.skv);  // every owned key takes part
+            while (st < u.t1) {
                 uint32_t live = 0xffffffffu;  // query pass: my columns' keys; key pass: all or nothing
-                if (!kKeys) {
+                if (whole && (kKeys || (st + 1) * kTileN <= p.skv)) {
+                } else if (!kKeys) {
                     live = static_cast<uint32_t>(x_key_word(p.words != nullptr ? p.words + static_cast<long long>(u.b) * n_words : nullptr,
                                                             p.skv, 2 * st + (piece >> 1)) >> ((piece & 1) * 32));
                 } else if (p.words != nullptr) {
@@ -476,9 +490,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 const bool plain = __all_sync(0xffffffffu, live == 0xffffffffu);
                 // (key pass: the step's statistics come with W)
                 const float4* cl = reinterpret_cast<const float4*>(stat + (j % kXWStages) * 2 * kTileN + piece * 32);
-                if (kKeys) ok = wait(&ctl->w_full[j % kXWStages], (j / kXWStages) & 1);
-                ok = ok && wait(&ctl->t1_full, j & 1);
-                if (!ok) break;
+                if (kKeys) ok = wait(&ctl->w_full[j % kXWStages], (j / kXWStages) & 1) && ok;
+                ok = wait(&ctl->t1_full, j & 1) && ok;
                 tc_fence_after();
                 uint32_t a[32];
                 tmem_ld32(t1, a);
@@ -520,8 +533,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                     tc_fence_before();
                     arrive(&ctl->p_full);
                 }
-                ok = wait(&ctl->t2_full, j & 1);
-                if (!ok) break;
+                ok = wait(&ctl->t2_full, j & 1) && ok;
                 tc_fence_after();
                 uint32_t d[32], ds[16];
                 tmem_ld32(t2, d);
@@ -552,79 +564,77 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 tc_fence_before();
                 arrive(&ctl->ds_full);
                 if (kKeys && lane == 0) mbar_arrive(smem_u32(&ctl->w_empty[j % kXWStages]));
+                if (!ok) break;
+                if (!kKeys) release_xy();  // (behind the first step: the stores have long been read by then)
+                ++j;
+                st = x_bwd_live<kKeys>(p, u, st + 1);
             }
             if (!ok) break;
             bool copied = false;
             if (any) {
-                ok = wait(&ctl->acc_done, n_seg & 1);
-                if (!ok) break;
-                tc_fence_after();
-                ++n_seg;
-                // (the next segment's first products run during this one's epilogue)
+                // The last T2 is there, so X and Y in TMEM are free: the next segment's first products follow this
+                // one's last in the tensor core's queue and run during this one's epilogue.
                 if (!kKeys && x_bwd_more<kKeys>(p, cursor)) {
                     ok = copy_xy();
                     if (!ok) break;
                     copied = true;
                 }
+                ok = wait(&ctl->acc_done, n_seg & 1);
+                // (the epilogue reuses the memory that X and Y were copied from: by all warps, first)
+                if (copied) ok = wait(&ctl->xt_full, (n_copied - 1) & 1) && ok;
+                if (!ok) break;
+                tc_fence_after();
+                ++n_seg;
             }
-            // Each warp writes 32 rows x 64 columns: the key pass's warps those of dk and dv, the query pass's
-            // first warps those of dq; staged where the owned tiles were, which are no longer needed.
-            const int which = kKeys ? piece / (kD / 64) : 0;
-            const int cb = kKeys ? piece % (kD / 64) : piece;  // 64-column block
-            if (which < 2 && cb < kD / 64) {
-                const uint32_t ta = tmem + lane_base + (which ? kColA2 : kColA1) + cb * 64;
-                const int row_w = u.tile * kTileM + quarter * 32;
-                uint8_t* stage = smem + warp * kXStageBytes;
-                const int rows = kKeys ? p.skv : p.sq;
+            // Each warp writes blocks of 32 rows x 32 columns: the query pass's one of dq, the key pass's two of dk and
+            // dv; staged where the owned tiles were, which are no longer needed.
+            constexpr int kBlocks = (kKeys ? 2 : 1) * kD / 32;  // of 32 columns
+            static_assert(kXBwdSoftWarps * ((kBlocks + 3) / 4) * kXStageBytes <= 2 * kTileBytes, "the staging fits");
+            const int row_w = u.tile * kTileM + quarter * 32, rows = kKeys ? p.skv : p.sq;
+#pragma unroll
+            for (int blk = piece; blk < kBlocks; blk += 4) {
+                const int which = blk / (kD / 32), col = blk % (kD / 32) * 32;
                 if (!any && seg.slot < 0) {
                     // nothing to add up: zeros, stored directly (the memory may hold the next owned tiles)
                     if (row < rows) {
-                        uint4* dst = reinterpret_cast<uint4*>(p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]) + cb * 64);
+                        uint4* dst = reinterpret_cast<uint4*>(p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]) + col);
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) dst[x] = make_uint4(0, 0, 0, 0);
+                        for (int x = 0; x < 4; ++x) dst[x] = make_uint4(0, 0, 0, 0);
                     }
+                    continue;
+                }
+                uint32_t o[32];
+                tmem_ld32(tmem + lane_base + (which ? kColA2 : kColA1) + col, o);
+                tc_wait_ld();
+                tmem_ld_fence(o);
+                if (!any) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+                }
+                if (seg.slot < 0) {
+                    uint8_t* stage = smem + (warp * 2 + blk / 4) * kXStageBytes;
+                    x_stage32<kBF16>(stage, lane, o, which ? 1.0f : p.scale);
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0 && row_w < rows)
+                        tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(stage), col, row_w, u.head, u.b, 0);
                 } else {
+                    float4* part = reinterpret_cast<float4*>(p.part) +
+                                   ((static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) + col / 4) * kTileM + row_in_tile;
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        uint32_t o[32];
-                        tmem_ld32(ta + b * 32, o);
-                        tc_wait_ld();
-                        tmem_ld_fence(o);
-                        if (!any) {
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) o[x] = 0u;
-                        }
-                        if (seg.slot < 0) {
-                            x_stage32<kBF16>(stage, lane, b, o, which ? 1.0f : p.scale);
-                        } else {
-                            float4* part = reinterpret_cast<float4*>(p.part) +
-                                           ((static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) + cb * 16 + b * 8) * kTileM + row_in_tile;
-#pragma unroll
-                            for (int v4 = 0; v4 < 8; ++v4)
-                                __stcg(part + v4 * kTileM,
-                                       make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
-                                                   __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
-                        }
-                    }
-                    if (seg.slot < 0) {
-                        fence_proxy_async_shared();
-                        __syncwarp();
-                        if (lane == 0 && row_w < rows)
-                            tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(stage), cb * 64, row_w, u.head, u.b, 0);
-                    }
+                    for (int v4 = 0; v4 < 8; ++v4)
+                        __stcg(part + v4 * kTileM,
+                               make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
+                                           __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
                 }
             }
             if (any) {
                 tc_fence_before();
                 arrive(&ctl->acc_free);
-                // the owned tiles' memory may be loaded again: key pass, the next ones; query pass, those behind
-                // the ones already copied
-                if (kKeys || copied) {
-                    if (lane == 0) {
-                        tma_store_wait_read();
-                        mbar_arrive(smem_u32(&ctl->xy_empty));
-                    }
-                }
+                // The owned tiles' memory may be loaded again: key pass, with the next ones; query pass, with those
+                // behind the ones already copied.
+                owe_release = kKeys || copied;
+                if (kKeys) release_xy();
             }
         }
         if (lane == 0) tma_store_wait();

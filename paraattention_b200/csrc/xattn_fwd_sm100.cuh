@@ -47,8 +47,8 @@ struct XFwdCtl {
     uint32_t tmem_base;
     int abort;
 };
-// alignment slack; Q, K and V ring; output staging of the 8 softmax warps; control block
-constexpr int kXFwdSmemBytes = 1024 + 6 * kTileBytes + kSoftmaxWarps * kXStageBytes + 512;
+// alignment slack; Q, K and V ring; output staging, two buffers for each softmax warp; control block
+constexpr int kXFwdSmemBytes = 1024 + 6 * kTileBytes + 2 * kSoftmaxWarps * kXStageBytes + 512;
 static_assert(kXFwdSmemBytes <= 232448, "shared memory");
 static_assert(sizeof(XFwdCtl) <= 512, "control block too large");
 
@@ -88,7 +88,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const uint32_t sQ = smem_u32(smem);
     const uint32_t sK = sQ + 2 * kTileBytes;
     const uint32_t sV = sK + 2 * kTileBytes;
-    XFwdCtl* ctl = reinterpret_cast<XFwdCtl*>(smem + 6 * kTileBytes + kSoftmaxWarps * kXStageBytes);
+    XFwdCtl* ctl = reinterpret_cast<XFwdCtl*>(smem + 6 * kTileBytes + 2 * kSoftmaxWarps * kXStageBytes);
     volatile int* s_abort = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -439,29 +439,26 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 continue;
             }
             const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;  // (no key at all: zeros, LSE -inf)
-            uint8_t* stage = smem + 6 * kTileBytes + warp * kXStageBytes;
+            uint8_t* stage = smem + 6 * kTileBytes + warp * (2 * kXStageBytes);
             const bool zero = n <= 0 || !(l_sum > 0.0f);
             const int row_w = (tile - g * p.mt) * kTileM + quarter * 32;  // first of the warp's rows
 #pragma unroll
-            for (int cb = 0; cb < kD / 64; ++cb) {
-                if (lane == 0) tma_store_wait_read();  // (the staging memory is free again)
+            for (int b = 0; b < kD / 32; ++b) {
+                uint32_t o[32];
+                tmem_ld32(tO + b * 32, o);
+                if (lane == 0) tma_store_wait_read<1>();  // (this buffer's last store has been read)
                 __syncwarp();
+                tc_wait_ld();
+                tmem_ld_fence(o);
+                if (zero) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t o[32];
-                    tmem_ld32(tO + cb * 64 + b * 32, o);
-                    tc_wait_ld();
-                    tmem_ld_fence(o);
-                    if (zero) {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = 0u;
-                    }
-                    x_stage32<kBF16>(stage, lane, b, o, inv);
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
                 }
+                x_stage32<kBF16>(stage + (b & 1) * kXStageBytes, lane, o, inv);
                 fence_proxy_async_shared();
                 __syncwarp();
                 if (lane == 0 && g < p.group && row_w < p.sq)
-                    tma_store_5d(&tm_o, smem_u32(stage), cb * 64, row_w, head, w.b, 0);
+                    tma_store_5d(&tm_o, smem_u32(stage + (b & 1) * kXStageBytes), b * 32, row_w, head, w.b, 0);
             }
             if (in_range && p.lse != nullptr)
                 p.lse[(static_cast<long long>(w.b) * p.hkv * p.group + head) * p.sq + row] =

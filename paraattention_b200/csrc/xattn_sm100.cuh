@@ -139,13 +139,13 @@ __device__ __forceinline__ void x_zero_rows(uint8_t* base, int atom_stride, unsi
         if (((word >> r) & 1ull) == 0) *reinterpret_cast<uint4*>(at + r * 128) = make_uint4(0, 0, 0, 0);
 }
 
-// Writes 32 rows x 64 columns of results, one row per lane (`o`: 64 fp32 values of the lane's row, in two
-// groups of 32, scaled by f) as 16-bit values to a warp's 4 KB of shared memory in the 128-byte
-// swizzle of a tensor map with boxes of 32 rows, from where one lane stores them with TMA: the 32 lanes
-// hold 32 different rows, so storing from registers touches 32 lines per instruction (measured: 8700
-// cycles for a 128 x 128 tile per warpgroup against about 900 this way).
+// Writes 32 rows x 32 columns of results, one row per lane (`o`: the fp32 values of the lane's row, scaled
+// by f) as 16-bit values to 2 KB of shared memory in the 64-byte swizzle of a tensor map with boxes of 32
+// x 32, from where one lane stores them with TMA: the 32 lanes hold 32 different rows, so storing from
+// registers touches 32 lines per instruction (measured in the forward kernel: 8700 cycles for a
+// 128 x 128 tile per warpgroup, against 2950 with TMA stores from one 4 KB buffer per warp).
 template <bool kBF16>
-__device__ __forceinline__ void x_stage32(uint8_t* stage, int lane, int group, const uint32_t (&o)[32], float f) {
+__device__ __forceinline__ void x_stage32(uint8_t* stage, int lane, const uint32_t (&o)[32], float f) {
 #pragma unroll
     for (int v4 = 0; v4 < 4; ++v4) {
         uint32_t q[4];
@@ -154,10 +154,9 @@ __device__ __forceinline__ void x_stage32(uint8_t* stage, int lane, int group, c
             const float a = __uint_as_float(o[v4 * 8 + 2 * x]) * f, b = __uint_as_float(o[v4 * 8 + 2 * x + 1]) * f;
             q[x] = kBF16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
         }
-        const int chunk = group * 4 + v4;
-        *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((v4 ^ ((lane >> 1) & 3)) << 4)) = make_uint4(q[0], q[1], q[2], q[3]);
     }
 }
-constexpr int kXStageBytes = 32 * 128;  // per warp
+constexpr int kXStageBytes = 32 * 64;
 
 }  // namespace pa
