@@ -198,6 +198,23 @@ def load() -> C.CDLL:
     return lib
 
 
+_torch_ext = None
+
+
+def load_torch_ext():
+    """The PyTorch extension of the differentiable operators (links to the library), imported once."""
+    global _torch_ext
+    if _torch_ext is None:
+        load()
+        try:
+            from . import _pa_torch
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `python -m paraattention_b200.build_ext`. There is no CPU or PyTorch "
+                              "fallback.") from e
+        _torch_ext = _pa_torch
+    return _torch_ext
+
+
 def check(rc: int) -> None:
     if rc != PA_OK:
         raise PaError(rc, load().pa_last_error().decode())
