@@ -17,6 +17,8 @@ __version__ = "0.1.0"
 
 from . import config, ops  # noqa: E402
 from .para_attn_interface import (  # noqa: E402
+    cross_attn_func,
+    CrossAttnMode,
     in_batch_attn_func,
     InBatchAttnMode,
     ring_attn_func,
@@ -37,6 +39,8 @@ __all__ = [
     "InBatchAttnMode",
     "SparseKVAttnMode",
     "sparse_kv_attn_func",
+    "CrossAttnMode",
+    "cross_attn_func",
     "ring_attn_func",
     "ulysses_attn_func",
     "in_batch_attn_func",

@@ -24,6 +24,9 @@ class attention:
     # the shape-only transformers of this package prepare q, k, v with the fused kernel
     # (ops.qkv_prepare) instead of a chain of tensor operations when their tensors allow it
     fuse_qkv_prepare = os.getenv("PA_B200_FUSE_QKV_PREPARE", "1") == "1"
+    # where gradients are recorded, they prepare q and k with the differentiable ops.qk_norm_rotary (one
+    # rounding where the eager chain has three); the fused kernel above carries no gradient
+    differentiable = os.getenv("PA_B200_DIFFERENTIABLE") == "1"
     # non-causal single-GPU attention launches whose last wave of CTAs would leave most SMs idle
     # give the work units of that wave to several CTAs each (the keys are split among them; the
     # library decides per shape). Costs one scratch buffer of 64 MB per device and stream.

@@ -32,6 +32,8 @@ __all__ = [
     "unified_attn_func",
     "sparse_kv_attn_func",
     "SparseKVAttnMode",
+    "cross_attn_func",
+    "CrossAttnMode",
 ]
 
 
@@ -425,3 +427,56 @@ class InBatchAttnMode(_AttnModeBase):
 
     def _call_attn_func(self, *args, **kwargs):
         return in_batch_attn_func(*args, **kwargs)
+
+
+def cross_attn_func(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False, *, scale=None, enable_gqa=False):
+    """``F.scaled_dot_product_attention`` for queries and keys of different lengths (text or image states
+    of an encoder), with gradients: ``ops.cross_attention`` behind that function's signature. No
+    counterpart in the reference, whose modes hand such calls back to PyTorch (``skip_small_kv``,
+    src/para_attn/para_attn_interface.py:303-345) or exchange the replicated keys between the ranks.
+
+    ``attn_mask``: a boolean key-padding mask, as in ``sparse_kv_attn_func``. With ``enable_gqa`` key and
+    value may have fewer heads than query."""
+    assert query.ndim == 4 and key.ndim == 4 and value.ndim == 4, "query, key and value must be [B, H, S, D]"
+    if dropout_p != 0.0:
+        raise NotImplementedError("cross_attn_func: dropout is not built")
+    if is_causal:
+        raise NotImplementedError("cross_attn_func: is_causal is not supported")
+    assert enable_gqa or key.shape[1] == query.shape[1], "key heads differ from query heads: pass enable_gqa=True"
+    key_mask = None
+    if attn_mask is not None:
+        key_mask = para_attn_ops.key_mask_of(attn_mask, query.shape[0], key.shape[2])
+        if key_mask is None:
+            raise NotImplementedError(
+                f"cross_attn_func: attn_mask of shape {tuple(attn_mask.shape)} is not a boolean key-padding mask "
+                f"broadcastable to [{query.shape[0]}, 1, 1, {key.shape[2]}]")
+    return para_attn_ops.cross_attention(query, key, value, key_mask, scale=scale)
+
+
+class CrossAttnMode(_AttnModeBase):
+    """Routes ``F.scaled_dot_product_attention`` calls whose keys are of another length than the queries
+    to ``cross_attn_func``; every other call passes. Under context parallelism, where each rank has its own
+    query rows and the whole prompt, such calls need no exchange: enter this mode outside a
+    ``UnifiedAttnMode(mesh, skip_small_kv=True)``, which hands them on.
+
+    ``same_length=True`` takes the self-attention calls too: the way to train a transformer block on one
+    GPU with this library's kernels (the other modes compute no gradients)."""
+
+    disabled = False
+
+    @torch.compiler.disable
+    def __init__(self, *, same_length=False):
+        super().__init__()
+        self._skip_small_kv = False
+        self._same_length = same_length
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        kwargs = {} if kwargs is None else kwargs
+        if func is F.scaled_dot_product_attention and not type(self).disabled and not self._same_length:
+            query, key = _get_args(args, kwargs, "query", "key")
+            if query.shape[-2] == key.shape[-2]:
+                return base_handle_torch_function(func, types, args, kwargs)
+        return super().__torch_function__(func, types, args, kwargs)
+
+    def _call_attn_func(self, *args, **kwargs):
+        return cross_attn_func(*args, **kwargs)

@@ -60,6 +60,9 @@ def _joint_qkv(streams, rotary, rotary_rows=None):
     ``rotary_rows = (first, count)`` limits the rotation to those rows of the joint sequence,
     table row 0 belonging to joint row ``first`` (default: all rows). Returns [B, H, sum S_i, D] views.
 
+    With ``config.attention.differentiable``, where a gradient is recorded, each stream goes through
+    ops.qk_norm_rotary, whose backward pass is a kernel too.
+
     On CUDA bf16/f16 tensors each stream is one launch of the fused kernel (three when only a
     part of it rotates), which normalises, rotates and writes into the joint buffers
     (``config.attention.fuse_qkv_prepare``); otherwise the same arithmetic runs as the chain of
@@ -69,6 +72,9 @@ def _joint_qkv(streams, rotary, rotary_rows=None):
     q0 = streams[0][0]
     total = sum(st[0].shape[1] for st in streams)
     first, count = (0, total) if rotary_rows is None else rotary_rows
+    if (config.attention.differentiable and torch.is_grad_enabled() and q0.device.type == "cuda"
+            and q0.dtype in (torch.bfloat16, torch.float16) and any(t is not None and t.requires_grad for st in streams for t in st)):
+        return _joint_qkv_differentiable(streams, rotary, first, count)
     if config.attention.fuse_qkv_prepare and q0.device.type == "cuda" and q0.dtype in (torch.bfloat16, torch.float16):
         from . import ops
 
@@ -110,6 +116,28 @@ def _joint_qkv(streams, rotary, rotary_rows=None):
             q = torch.cat([q[:, :, :first], _rope(q[:, :, sl], cos, sin), q[:, :, first + count:]], dim=2)
             k = torch.cat([k[:, :, :first], _rope(k[:, :, sl], cos, sin), k[:, :, first + count:]], dim=2)
     return q, k, v
+
+
+def _joint_qkv_differentiable(streams, rotary, first, count):
+    """``_joint_qkv`` with gradients: norm and rotation of each stream as one call (three when only a part
+    of it rotates), and concatenations."""
+    from . import ops
+
+    qs, ks, vs = [], [], []
+    off = 0
+    for q, k, v, wq, wk in streams:
+        rows = q.shape[1]
+        lo, hi = max(off, first) - off, min(off + rows, first + count) - off  # rows of this stream that rotate
+        cuts = [(0, rows, False)] if rotary is None or hi <= lo else [(0, lo, False), (lo, hi, True), (hi, rows, False)]
+        for a, b, rotate in cuts:
+            if b > a:
+                yq, yk = ops.qk_norm_rotary(_split_heads(q[:, a:b]), _split_heads(k[:, a:b]), wq, wk,
+                                            rotary if rotate else None, row_offset=off + a - first if rotate else 0)
+                qs.append(yq)
+                ks.append(yk)
+        vs.append(_split_heads(v))
+        off += rows
+    return tuple(torch.cat(t, dim=2) if len(t) > 1 else t[0] for t in (qs, ks, vs))
 
 
 def _rope_table(positions: torch.Tensor, axes_dim=(16, 56, 56), theta: float = 10000.0):
