@@ -55,12 +55,18 @@ int run_few(const pa_xattn_args* a, cudaStream_t s) {
     p.skv = a->seq_kv;
     p.scale = a->scale;
     p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.status = a->status;
+    p.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     // CTAs per (batch, kv head): as many as it takes to fill the GPU with two resident CTAs per SM,
     // as long as each has a key tile.
     const long long units = static_cast<long long>(a->batch) * a->kv_heads;
     const int tiles = (a->seq_kv + pa::kFewKeys - 1) / pa::kFewKeys;
     int c = 1;
+#ifdef PA_FEW_C
+    while (c < PA_FEW_C && 2 * c <= tiles) c *= 2;
+#else
     while (c < pa::kFewMaxCluster && units * c < 2ll * sm_count() && 2 * c <= tiles) c *= 2;
+#endif
     auto kern = pa::xattn_few_kernel<kBF16, kD>;
     const int smem = pa::few_smem_bytes<kD>();
     const int rc = allow_smem(kern, smem, "xattn few rows");
@@ -68,7 +74,7 @@ int run_few(const pa_xattn_args* a, cudaStream_t s) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(units * c));
-    cfg.blockDim = dim3(pa::kFewThreads);
+    cfg.blockDim = dim3(2 * pa::kFewThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr;

@@ -8,9 +8,11 @@
 //
 // One cluster of 1, 2, 4 or 8 CTAs per (batch, kv head), the key tiles of 64 divided among its CTAs,
 // so that few heads still fill the GPU in ONE launch: the CTAs' partial results are joined through
-// distributed shared memory. Inside a CTA each of 4 warps owns 16 keys of every tile; K and V go
-// through a 3-stage cp.async ring. Keys that are masked or behind the last are not read: their
-// copy fills zeros (so infinities or NaN there never enter) and their logits are -inf.
+// distributed shared memory. Inside a CTA each of 4 warps owns 16 keys of every tile; 4 other warps
+// fill a 3-stage cp.async ring with K and V (the copies' addresses and the mask cost as many
+// instructions as the arithmetic: one set of warps doing both in turn took 2.6 us per tile with two
+// CTAs on an SM, four times what HBM needs). Keys that are masked or behind the last are not
+// read: their copy fills zeros (so infinities or NaN there never enter) and their logits are -inf.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -24,7 +26,7 @@ namespace pa {
 
 constexpr int kFewRows = 16;
 constexpr int kFewKeys = 64;
-constexpr int kFewThreads = 128;
+constexpr int kFewThreads = 128;  // that compute; as many more load
 constexpr int kFewStages = 3;
 constexpr int kFewMaxCluster = 8;
 
@@ -37,12 +39,14 @@ struct XFewParams {
     long long mask_s;
     int hkv, group, sq, skv;
     float scale, scale_log2;
+    int* status;
+    unsigned long long wait_ns;
 };
 
 template <int kD>
 constexpr int few_smem_bytes() {
-    // Q tile, ring of K and V tiles with their key flags; (the ring is reused for the joining)
-    return kFewRows * kD * 2 + kFewStages * (2 * kFewKeys * kD * 2 + kFewKeys) + 4 * kFewRows * 8 + kFewRows * 8 + 16;
+    // Q tile, ring of K and V tiles (reused for the joining), row statistics, barriers
+    return kFewRows * kD * 2 + kFewStages * 2 * kFewKeys * kD * 2 + 5 * kFewRows * 8 + 2 * kFewStages * 8 + 16;
 }
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool live) {
@@ -74,64 +78,87 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 template <bool kBF16, int kD>
-__global__ void __launch_bounds__(kFewThreads)
+__global__ void __launch_bounds__(2 * kFewThreads)
 xattn_few_kernel(const __grid_constant__ XFewParams p) {
     namespace cg = cooperative_groups;
     constexpr int kChunks = kD / 8;                 // 16-byte chunks of a row
     constexpr int kRowBytes = kD * 2;
     constexpr int kTile = kFewKeys * kRowBytes;     // bytes of a K or V tile
-    constexpr int kStage = 2 * kTile + kFewKeys;    // K, V, key flags
+    constexpr int kStage = 2 * kTile;               // K, V
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* sq_ = smem;
     uint8_t* ring = smem + kFewRows * kRowBytes;
     float2* wml = reinterpret_cast<float2*>(ring + kFewStages * kStage);  // [4 warps][16 rows]
     float2* cml = wml + 4 * kFewRows;                                     // [16 rows] of this CTA
 
+    uint64_t* full = reinterpret_cast<uint64_t*>(cml + kFewRows);         // [stages], one arrival per loading thread
+    uint64_t* empty = full + kFewStages;                                  // [stages], one arrival per computing warp
+    int* abort_word = reinterpret_cast<int*>(empty + kFewStages);
+    volatile int* s_abort = abort_word;
+
     auto cluster = cg::this_cluster();
     const int cn = static_cast<int>(cluster.num_blocks()), cr = static_cast<int>(cluster.block_rank());
     const int unit = blockIdx.x / cn;
     const int hk = unit % p.hkv, b = unit / p.hkv;
     const int rows = p.group * p.sq;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x % kFewThreads, lane = tid & 31, warp = tid >> 5;
+    const bool loader = threadIdx.x >= kFewThreads;
     const int tiles = (p.skv + kFewKeys - 1) / kFewKeys;
     const int tile0 = static_cast<int>(static_cast<long long>(tiles) * cr / cn);
     const int tile1 = static_cast<int>(static_cast<long long>(tiles) * (cr + 1) / cn);
-
-    const uint16_t* kb = p.k + b * p.k_s[0] + hk * p.k_s[1];
-    const uint16_t* vb = p.v + b * p.v_s[0] + hk * p.v_s[1];
     const uint8_t* mb = p.mask != nullptr ? p.mask + b * p.mask_s : nullptr;
 
-    const int my_chunk = tid % kChunks, my_key = tid / kChunks;
-    constexpr int kKeysPerPass = kFewThreads / kChunks, kPasses = kFewKeys / kKeysPerPass;
-    auto load = [&](int tile, int stage) {
-        uint8_t* st = ring + stage * kStage;
-        bool keep[kPasses];
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int key = tile * kFewKeys + my_key + i * kKeysPerPass;
-            keep[i] = tile < tile1 && key < p.skv && (mb == nullptr || __ldg(mb + key) != 0);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kFewStages; ++i) {
+            mbar_init(smem_u32(full + i), kFewThreads);
+            mbar_init(smem_u32(empty + i), kFewThreads / 32);
         }
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int r = my_key + i * kKeysPerPass;
-            const long long key = keep[i] ? tile * kFewKeys + r : 0;
-            const uint32_t at = r * kRowBytes + ((my_chunk ^ (r & 7)) << 4);
-            cp_async16_zfill(smem_u32(st + at), kb + key * p.k_s[2] + my_chunk * 8, keep[i]);
-            cp_async16_zfill(smem_u32(st + kTile + at), vb + key * p.v_s[2] + my_chunk * 8, keep[i]);
-            if (my_chunk == 0) st[2 * kTile + r] = keep[i] ? 1 : 0;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+        *abort_word = 0;
+        mbar_init_fence();
+    }
     // Q rows: row r = (head r / Sq of the group, query r % Sq); rows that do not exist are zeros
-    for (int i = tid; i < kFewRows * kChunks; i += kFewThreads) {
+    for (int i = threadIdx.x; i < kFewRows * kChunks; i += 2 * kFewThreads) {
         const int r = i / kChunks, c = i % kChunks;
         const bool live = r < rows;
         const int g = live ? r / p.sq : 0, s = live ? r - g * p.sq : 0;
         const uint16_t* src = p.q + b * p.q_s[0] + (hk * p.group + g) * p.q_s[1] + s * p.q_s[2] + c * 8;
-        cp_async16_zfill(smem_u32(sq_ + r * kRowBytes + ((c ^ (r & 7)) << 4)), src, live);
+        *reinterpret_cast<uint4*>(sq_ + r * kRowBytes + ((c ^ (r & 7)) << 4)) =
+            live ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
     }
+    __syncthreads();
+
+    if (loader) {
+        constexpr int kKeysPerPass = kFewThreads / kChunks, kPasses = kFewKeys / kKeysPerPass;
+        const int my_chunk = tid % kChunks, my_key = tid / kChunks;
+        const uint16_t* kb = p.k + b * p.k_s[0] + hk * p.k_s[1] + my_chunk * 8;
+        const uint16_t* vb = p.v + b * p.v_s[0] + hk * p.v_s[1] + my_chunk * 8;
+        for (int t = tile0, n = 0; t < tile1; ++t, ++n) {
+            bool keep[kPasses];
 #pragma unroll
-    for (int s = 0; s < kFewStages - 1; ++s) load(tile0 + s, s);  // (the first group holds Q too)
+            for (int i = 0; i < kPasses; ++i) {
+                const int key = t * kFewKeys + my_key + i * kKeysPerPass;
+                keep[i] = key < p.skv;
+                if (mb != nullptr) keep[i] = keep[i] & (__ldg(mb + min(key, p.skv - 1)) != 0);
+            }
+            const int st = n % kFewStages;
+            if (n >= kFewStages &&
+                !mbar_wait(smem_u32(empty + st), ((n / kFewStages) & 1) ^ 1, s_abort, p.status, p.wait_ns, PA_DEV_TIMEOUT_PIPE))
+                break;
+            const uint32_t base = smem_u32(ring + st * kStage);
+            const uint16_t* kt = kb + static_cast<long long>(t) * kFewKeys * p.k_s[2];
+            const uint16_t* vt = vb + static_cast<long long>(t) * kFewKeys * p.v_s[2];
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                const int r = my_key + i * kKeysPerPass;
+                const uint32_t at = r * kRowBytes + ((my_chunk ^ (r & 7)) << 4);
+                // (a copy of zero bytes reads nothing; its address stays inside the tensor all the same)
+                cp_async16_zfill(base + at, keep[i] ? kt + r * p.k_s[2] : kb, keep[i]);
+                cp_async16_zfill(base + kTile + at, keep[i] ? vt + r * p.v_s[2] : vb, keep[i]);
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(full + st)) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
 
     float o[kChunks][4];
 #pragma unroll
@@ -142,21 +169,30 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
     uint32_t qa[kD / 16][4];
     const float sl = p.scale_log2;
 
-    for (int t = tile0, n = 0; t < tile1; ++t, ++n) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kFewStages - 2) : "memory");
-        __syncthreads();
-        load(t + kFewStages - 1, (n + kFewStages - 1) % kFewStages);
-        if (n == 0) {
+    // Which of my warp's 16 keys of a tile take part: the byte is looked at a tile ahead.
+    auto look = [&](int t) -> uint32_t {
+        const int key = t * kFewKeys + warp * 16 + (lane & 15);
+        return key < p.skv ? (mb != nullptr ? static_cast<uint32_t>(__ldg(mb + key)) : 1u) : 0u;
+    };
+    uint32_t next = loader ? 0u : look(tile0);
+    if (!loader) {
 #pragma unroll
-            for (int ks = 0; ks < kD / 16; ++ks) {
-                const int r = lane & 15, c = 2 * ks + (lane >> 4);
-                ldsm4(smem_u32(sq_ + r * kRowBytes + ((c ^ (r & 7)) << 4)), qa[ks]);
-            }
+        for (int ks = 0; ks < kD / 16; ++ks) {
+            const int r = lane & 15, c = 2 * ks + (lane >> 4);
+            ldsm4(smem_u32(sq_ + r * kRowBytes + ((c ^ (r & 7)) << 4)), qa[ks]);
         }
-        uint8_t* st = ring + (n % kFewStages) * kStage;
-        const uint8_t* flags = st + 2 * kTile + warp * 16;
-        const uint4 f = *reinterpret_cast<const uint4*>(flags);
-        if ((f.x | f.y | f.z | f.w) == 0) continue;  // no key of this warp's 16 takes part
+    }
+    for (int t = tile0, n = 0; t < tile1 && !loader; ++t, ++n) {
+        const uint32_t live = __ballot_sync(0xffffffffu, next != 0) & 0xffffu;
+        next = look(t + 1);
+        const int slot = n % kFewStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(full + slot), (n / kFewStages) & 1, s_abort, p.status, p.wait_ns, PA_DEV_TIMEOUT_PIPE)))
+            break;
+        uint8_t* st = ring + slot * kStage;
+        if (live == 0) {  // no key of this warp's 16 takes part
+            if (lane == 0) mbar_arrive(smem_u32(empty + slot));
+            continue;
+        }
         float s[2][4];
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
@@ -176,7 +212,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int col = nb * 8 + (lane & 3) * 2 + (i & 1);
-                s[nb][i] = flags[col] != 0 ? s[nb][i] * sl : -INFINITY;
+                s[nb][i] = ((live >> col) & 1u) != 0 ? s[nb][i] * sl : -INFINITY;
                 mx[i >> 1] = fmaxf(mx[i >> 1], s[nb][i]);
             }
         float alpha[2];
@@ -214,13 +250,15 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
             mma16816<kBF16>(o[c], pa_, vf[0], vf[1]);
             mma16816<kBF16>(o[c + 1], pa_, vf[2], vf[3]);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(empty + slot));
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
     // ---- join the 4 warps: O [warp][16][kD] fp32 over the ring ------------------------------------
     float* wo = reinterpret_cast<float*>(ring);
     static_assert(4 * kFewRows * kD * 4 <= kFewStages * kStage, "the ring holds the partial results");
+    if (!loader) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -232,10 +270,11 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
             *reinterpret_cast<float2*>(wo + (warp * kFewRows + r) * kD + c * 8 + (lane & 3) * 2) =
                 make_float2(o[c][2 * h], o[c][2 * h + 1]);
     }
+    }
     __syncthreads();
-    constexpr int kPer = kFewRows * kD / kFewThreads;  // elements per thread, all of one row
+    constexpr int kPer = kFewRows * kD / (2 * kFewThreads);  // elements per thread, all of one row
     {
-        const int r = tid * kPer / kD, c0 = tid * kPer % kD;
+        const int r = threadIdx.x * kPer / kD, c0 = threadIdx.x * kPer % kD;
         float mt = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; ++w) mt = fmaxf(mt, wml[w * kFewRows + r].x);
@@ -265,7 +304,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
     // ---- join the CTAs of the cluster: 8 output elements per thread -----------------------------------
     if (cn > 1) cluster.sync();
     else __syncthreads();
-    for (int i = cr * kFewThreads + tid; i < rows * kChunks; i += cn * kFewThreads) {
+    for (int i = cr * 2 * kFewThreads + threadIdx.x; i < rows * kChunks; i += cn * 2 * kFewThreads) {
         const int r = i / kChunks, c0 = (i % kChunks) * 8;
         float mt = -INFINITY, lt = 0.f;
         for (int k = 0; k < cn; ++k) mt = fmaxf(mt, cluster.map_shared_rank(cml, k)[r].x);
