@@ -267,6 +267,7 @@ typedef struct pa_xattn_args {
     const uint8_t* key_mask;
     int64_t mask_stride;
     int32_t* status;
+    int32_t* status_host;    /* host memory the device can write (pinned), or NULL: receives the code too */
     uint64_t wait_limit_ns;
     void* workspace;
     int64_t workspace_bytes;

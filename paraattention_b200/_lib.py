@@ -113,7 +113,7 @@ class XattnArgs(C.Structure):
         ("o_stride", C.c_int64 * 3), ("do_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3),
         ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
         ("key_mask", C.c_void_p), ("mask_stride", C.c_int64),
-        ("status", C.c_void_p), ("wait_limit_ns", C.c_uint64),
+        ("status", C.c_void_p), ("status_host", C.c_void_p), ("wait_limit_ns", C.c_uint64),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
     ]
 

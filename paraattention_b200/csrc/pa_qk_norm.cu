@@ -16,7 +16,7 @@ namespace {
 
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 
-int max_ctas(bool backward) { return sm_count() * (backward ? pa::kQkNormCtasPerSm<true> : pa::kQkNormCtasPerSm<false>); }
+int max_ctas() { return sm_count() * pa::kQkNormCtasPerSm; }
 
 int fill(const pa_qk_norm_args* a, bool backward, pa::QkNormParams* p) {
     if (a == nullptr) return fail(PA_EINVAL, "qk_norm: args is NULL");
@@ -57,17 +57,24 @@ int fill(const pa_qk_norm_args* a, bool backward, pa::QkNormParams* p) {
     p->batch = a->batch;
     p->rows = a->rows;
     p->eps = a->eps;
-    // A row's heads stay with one warp (which loads the row's cos / sin once) as long as the rows
-    // fill the GPU; with fewer rows they are divided over several warps, down to one pass of the
-    // warp's lanes each.
+    // Shares of a row's heads: enough to occupy every warp, and such that the items fill the last round of
+    // warps well (4608 rows on 2368 warps: two rounds of whole rows do the
+    // work of 1.95; 2500 rows, of 1.06). A share costs about a head vector's time of its own
+    // (tables, addresses), and is never less than one warp-wide access.
     const long long lines = static_cast<long long>(a->batch) * a->rows;
-    const long long warps = static_cast<long long>(max_ctas(backward)) * pa::kQkNormWarps;
+    const long long warps = static_cast<long long>(max_ctas()) * pa::kQkNormWarps;
     const int vec = 256 / a->head_dim;  // head vectors of one warp-wide access
     const int most = (std::max(p->heads[0], p->heads[1]) + vec - 1) / vec;
-    long long chunks = warps / lines;
-    if (chunks > most) chunks = most;
-    if (chunks < 1) chunks = 1;
-    p->chunks = static_cast<int>(chunks);
+    double best = 0;
+    for (int c = 1; c <= most; ++c) {
+        const long long rounds = (lines * c + warps - 1) / warps;
+        const double turns = std::ceil(double(p->heads[0]) / c / vec) + std::ceil(double(p->heads[1]) / c / vec);
+        const double t = double(rounds) * (turns + 1.0);
+        if (c == 1 || t < best * 0.98) {
+            best = t;
+            p->chunks = c;
+        }
+    }
     return PA_OK;
 }
 
@@ -92,23 +99,23 @@ int run(const pa_qk_norm_args* a, const pa::QkNormParams& p, int grid, cudaStrea
     return PA_OK;
 }
 
-int grid_of(const pa::QkNormParams& p, bool backward) {
+int grid_of(const pa::QkNormParams& p) {
     const long long items = static_cast<long long>(p.batch) * p.rows * p.chunks;
     const long long ctas = (items + pa::kQkNormWarps - 1) / pa::kQkNormWarps;
-    return static_cast<int>(std::min<long long>(ctas, max_ctas(backward)));
+    return static_cast<int>(std::min<long long>(ctas, max_ctas()));
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t pa_qk_norm_workspace_bytes(void) { return static_cast<int64_t>(max_ctas(true)) * 2 * 128 * sizeof(float); }
+int64_t pa_qk_norm_workspace_bytes(void) { return static_cast<int64_t>(max_ctas()) * 2 * 128 * sizeof(float); }
 
 int pa_qk_norm_fwd(const pa_qk_norm_args* a, void* stream) {
     pa::QkNormParams p;
     const int rc = fill(a, false, &p);
     if (rc != PA_OK) return rc;
-    return run<false>(a, p, grid_of(p, false), static_cast<cudaStream_t>(stream));
+    return run<false>(a, p, grid_of(p), static_cast<cudaStream_t>(stream));
 }
 
 int pa_qk_norm_bwd(const pa_qk_norm_args* a, void* stream) {
@@ -116,7 +123,7 @@ int pa_qk_norm_bwd(const pa_qk_norm_args* a, void* stream) {
     int rc = fill(a, true, &p);
     if (rc != PA_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int grid = grid_of(p, true);
+    const int grid = grid_of(p);
     const bool weights = (a->dweight[0] != nullptr && a->weight[0] != nullptr) ||
                          (a->dweight[1] != nullptr && a->weight[1] != nullptr && a->x[1] != nullptr);
     if (weights) {

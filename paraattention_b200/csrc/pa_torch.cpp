@@ -10,8 +10,6 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
-#include <cuda_runtime_api.h>
-
 #include <optional>
 #include <string>
 #include <tuple>
@@ -64,7 +62,8 @@ void* stream_of(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.devi
 
 // ---- cross attention -----------------------------------------------------------------------------
 
-// The device's status word and its pinned mirror (block_ops.py passes their addresses; 0: none).
+// The device's status word and its pinned mirror, which these kernels write themselves when a wait gives up
+// (block_ops.py passes their addresses; 0: none).
 struct Status {
     int64_t word, host;
 };
@@ -108,6 +107,7 @@ void launch_cross(pa_xattn_args& a, bool backward, const Tensor& q, Status st) {
             throw PaFailure{PA_ETIMEDOUT, msg};
         }
         a.status = reinterpret_cast<int32_t*>(st.word);
+        a.status_host = reinterpret_cast<int32_t*>(st.host);
     }
     const int64_t n = pa_xattn_workspace_bytes(&a, backward ? 1 : 0);
     if (n < 0) raise(static_cast<int>(n), backward);
@@ -119,10 +119,6 @@ void launch_cross(pa_xattn_args& a, bool backward, const Tensor& q, Status st) {
     }
     void* stream = stream_of(q);
     check(backward ? pa_xattn_bwd(&a, stream) : pa_xattn_fwd(&a, stream), backward);
-    // (the kernel for few rows waits for nothing)
-    if (st.host != 0 && (backward || static_cast<int64_t>(a.heads / a.kv_heads) * a.seq_q > 16))
-        cudaMemcpyAsync(reinterpret_cast<void*>(st.host), reinterpret_cast<void*>(st.word), 4, cudaMemcpyDeviceToHost,
-                        static_cast<cudaStream_t>(stream));
 }
 
 std::tuple<Tensor, Tensor> cross_forward(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& rows,

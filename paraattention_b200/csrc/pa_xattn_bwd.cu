@@ -17,9 +17,9 @@ BwdPlan plan(const pa_xattn_args* a) {
     f.mt = (a->seq_q + 127) / 128;
     f.kt = (a->seq_kv + 127) / 128;
     const int sms = sm_count();
-    f.q = xattn_schedule(static_cast<long long>(a->batch) * a->heads * f.mt, f.kt, sms, 4, &f.grid_q);
+    f.q = xattn_schedule(static_cast<long long>(a->batch) * a->heads * f.mt, f.kt, 1, sms, 4, &f.grid_q);
     f.k = xattn_schedule(static_cast<long long>(a->kv_batch) * a->kv_heads * f.kt,
-                         static_cast<long long>(a->batch / a->kv_batch) * (a->heads / a->kv_heads) * f.mt, sms, 4, &f.grid_k);
+                         static_cast<long long>(a->batch / a->kv_batch) * (a->heads / a->kv_heads) * f.mt, f.kt, sms, 4, &f.grid_k);
     f.off_stats = xattn_mask_layout(a).bytes;
     f.off_part = f.off_stats + int64_t(a->batch) * a->heads * f.mt * 128 * 8;
     // (the passes run one after the other and use the same partial results' space)
@@ -36,8 +36,8 @@ int pass(const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& z, const
     if (rc != PA_OK) return rc;
     kern<<<grid, pa::kXBwdThreads, pa::kXBwdSmemBytes, s>>>(x, y, z, w, g0, g1, p);
     rc = launched("xattn backward");
-    if (rc != PA_OK || !p.sched.split) return rc;
-    pa::xattn_bwd_join_kernel<kBF16, kD, kKeys><<<dim3(p.sched.units, kD / 32, kKeys ? 2 : 1), 128, 0, s>>>(p, grid);
+    if (rc != PA_OK || !p.sched.split || grid == p.sched.team) return rc;
+    pa::xattn_bwd_join_kernel<kBF16, kD, kKeys><<<dim3(grid - p.sched.team, kD / 8, kKeys ? 2 : 1), 128, 0, s>>>(p, grid);
     return launched("xattn backward join");
 }
 
@@ -68,6 +68,7 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     p.stats = reinterpret_cast<float*>(ws + f.off_stats);
     p.part = reinterpret_cast<float*>(ws + f.off_part);
     p.status = a->status;
+    p.status_host = a->status_host;
     p.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     if (a->key_mask != nullptr) {
         p.words = reinterpret_cast<unsigned long long*>(ws);
@@ -92,7 +93,7 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     st.heads = a->heads;
     st.sq = a->seq_q;
     st.padded = f.mt * 128;
-    const long long vectors = static_cast<long long>(a->batch) * a->heads * st.padded, per_cta = pa::kXStatThreads / (kD / 8);
+    const long long vectors = static_cast<long long>(a->batch) * a->heads * st.padded, per_cta = pa::kXStatThreads / (kD / 8) * 4;
     const int stat_grid = static_cast<int>(std::min<long long>((vectors + per_cta - 1) / per_cta, 8ll * sm_count()));
     pa::xattn_stat_kernel<kBF16, kD><<<stat_grid, pa::kXStatThreads, 0, s>>>(st);
     rc = launched("xattn row statistics");

@@ -24,7 +24,7 @@ FwdPlan plan(const pa_xattn_args* a) {
     f.mt = (a->seq_q + 127) / 128;
     const long long tiles = static_cast<long long>(a->heads / a->kv_heads) * f.mt;
     const long long units = (tiles + 1) / 2 * a->kv_heads * a->batch;
-    f.sched = xattn_schedule(units, (a->seq_kv + 127) / 128, sm_count(), 4, &f.grid);
+    f.sched = xattn_schedule(units, (a->seq_kv + 127) / 128, 1, sm_count(), 4, &f.grid);
     const int64_t mask = xattn_mask_layout(a).bytes;
     f.off_ml = mask;
     f.off_o = f.off_ml + (f.sched.split ? int64_t(f.grid) * 2 * 256 * 8 : 0);
@@ -56,6 +56,7 @@ int run_few(const pa_xattn_args* a, cudaStream_t s) {
     p.scale = a->scale;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.status = a->status;
+    p.status_host = a->status_host;
     p.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     // CTAs per (batch, kv head): as many as it takes to fill the GPU with two resident CTAs per SM,
     // as long as each has a key tile.
@@ -114,6 +115,7 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     p.o_ss = a->o_stride[2];
     p.sched = f.sched;
     p.status = a->status;
+    p.status_host = a->status_host;
     p.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     if (a->key_mask != nullptr) {
@@ -134,8 +136,8 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     if (rc != PA_OK) return rc;
     kern<<<f.grid, pa::kAttnThreads, pa::kXFwdSmemBytes, s>>>(mq, mk, mv, mo, p);
     rc = launched("xattn forward");
-    if (rc != PA_OK || !f.sched.split) return rc;
-    pa::xattn_fwd_join_kernel<kBF16, kD><<<dim3(f.sched.units, kD / 32), 256, 0, s>>>(p, f.grid);
+    if (rc != PA_OK || !f.sched.split || f.grid == f.sched.team) return rc;
+    pa::xattn_fwd_join_kernel<kBF16, kD><<<dim3(f.grid - f.sched.team, kD / 8), 256, 0, s>>>(p, f.grid);
     return launched("xattn forward join");
 }
 

@@ -42,15 +42,18 @@ inline int xattn_sizes(const pa_xattn_args* a) {
 
 // Whole units or equal ranges of steps (see XSched)? Whole units take ceil(units / CTAs) rounds of
 // `steps` steps; ranges take units * steps / CTAs steps plus what the partial results cost,
-// `extra` steps' time.
-inline pa::XSched xattn_schedule(long long units, long long steps, int sms, int extra, int* grid) {
+// `extra` steps' time and a thirty-second of the whole. `shared`: consecutive units that walk the same streamed tiles; they form teams
+// unless that leaves more than one SM in sixteen without work.
+inline pa::XSched xattn_schedule(long long units, long long steps, int shared, int sms, int extra, int* grid) {
     pa::XSched s;
     s.units = static_cast<int>(units);
     s.steps = static_cast<int>(steps);
-    s.total = units * steps;
-    const long long whole = (units + sms - 1) / sms * steps, ranges = (s.total + sms - 1) / sms;
-    s.split = whole > ranges + extra ? 1 : 0;
-    *grid = static_cast<int>(std::min<long long>(sms, s.split ? s.total : units));
+    const long long all = units * steps;
+    const long long whole = (units + sms - 1) / sms * steps, ranges = (all + sms - 1) / sms;
+    s.split = whole - whole / 32 > ranges + extra ? 1 : 0;
+    s.team = s.split && shared > 1 && shared <= sms && sms / shared * shared * 16 >= sms * 15 ? shared : 1;
+    s.total = all / s.team;
+    *grid = static_cast<int>(s.split ? std::min<long long>(sms / s.team, s.total) * s.team : std::min<long long>(sms, units));
     return s;
 }
 

@@ -11,10 +11,11 @@
 //
 // HBM-bound: forward moves 4 bytes per element, backward 6. A lane owns 8 consecutive elements
 // (one 16-byte access), D / 8 lanes own a vector, so a warp works on 2 (D = 128) or 4 (D = 64)
-// heads of one row at a time with several loads in flight. A warp keeps the row's cos / sin
-// (fp32, 16 registers) and the weights across all heads it works on: re-reading the tables for
-// every head would move four times as many bytes through L1 as the data itself. A row's heads are
-// divided over several warps only when there are too few rows to fill the GPU.
+// heads of one row at a time, and the next turn's loads are issued before the last turn's
+// arithmetic. A warp keeps the row's cos / sin (fp32, 16 registers) and the weights across the heads it
+// works on: re-reading the tables for every head would move four times as many bytes through L1 as the
+// data itself. An item of work is a row and a share of its heads of q, then of k; the host chooses how
+// many shares so that the items fill whole rounds of warps.
 //
 // The weight gradients are summed in registers by each lane over all its heads and rows, then
 // over the CTA in a fixed order; a second small kernel adds the CTAs' partial sums in a fixed
@@ -30,9 +31,10 @@ namespace pa {
 
 constexpr int kQkNormThreads = 256;
 constexpr int kQkNormWarps = kQkNormThreads / 32;
-// (registers decide: the backward pass keeps the weight gradients of both tensors)
-template <bool kBackward>
-constexpr int kQkNormCtasPerSm = kBackward ? 2 : 3;
+// Resident CTAs per SM and vectors per lane and turn, by measurement (32760 rows of 80 heads of 128): forward 243 us
+// with 2 and 4 (250 with 3 and 2, 284 with 4 and 1), backward, whose weight gradients and second input
+// take registers, 383 us with 2 and 2 (405 with 2 and 3, 431 with 3 and 1, 556 with 1 and 4).
+constexpr int kQkNormCtasPerSm = 2;
 
 struct QkNormParams {
     const uint16_t* x[2];   // q, k (k may be NULL)
@@ -98,7 +100,7 @@ __device__ __forceinline__ float group_sum(float s) {
 }
 
 template <bool kBF16, int kD, bool kAdjacent, bool kBackward>
-__global__ void __launch_bounds__(kQkNormThreads, kQkNormCtasPerSm<kBackward>)
+__global__ void __launch_bounds__(kQkNormThreads, kQkNormCtasPerSm)
 qk_norm_kernel(const __grid_constant__ QkNormParams p) {
     constexpr int kLanes = kD / 8;       // lanes per vector
     constexpr int kVec = 32 / kLanes;    // vectors a warp works on at a time
@@ -146,22 +148,36 @@ qk_norm_kernel(const __grid_constant__ QkNormParams p) {
             const uint16_t* xb = p.x[t] + b * p.x_s[t][0] + row * p.x_s[t][1] + at;
             const uint16_t* gb = kBackward ? p.dy[t] + b * p.dy_s[t][0] + row * p.dy_s[t][1] + at : nullptr;
             uint16_t* yb = p.y[t] + b * p.y_s[t][0] + row * p.y_s[t][1] + at;
-            for (int base = h0; base < h1; base += kVec * kUnroll) {
-                uint4 xr[kUnroll], gr[kUnroll];
+            // (kUnroll vectors per lane in flight while as many are worked on)
+            uint4 xr[kUnroll], gr[kUnroll];
+            auto fetch = [&](int base) {
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u) {
                     const int h = base + u * kVec + sub;
-                    const bool live = h < h1;
-                    xr[u] = live ? __ldcs(reinterpret_cast<const uint4*>(xb + h * p.x_s[t][2])) : make_uint4(0, 0, 0, 0);
-                    if (kBackward)
-                        gr[u] = live ? __ldcs(reinterpret_cast<const uint4*>(gb + h * p.dy_s[t][2])) : make_uint4(0, 0, 0, 0);
+                    if (h < h1) {
+                        xr[u] = __ldcs(reinterpret_cast<const uint4*>(xb + h * p.x_s[t][2]));
+                        if (kBackward) gr[u] = __ldcs(reinterpret_cast<const uint4*>(gb + h * p.dy_s[t][2]));
+                    }
                 }
+            };
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) xr[u] = gr[u] = make_uint4(0, 0, 0, 0);
+            fetch(h0);
+            for (int base = h0; base < h1; base += kVec * kUnroll) {
+                uint4 xc[kUnroll], gc[kUnroll];
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    xc[u] = xr[u];
+                    gc[u] = gr[u];
+                }
+                fetch(base + kVec * kUnroll);
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u) {
                     if (base + u * kVec >= h1) break;  // (the same for the whole warp)
                     const int h = base + u * kVec + sub;
+                    const bool live = h < h1;
                     float x[8], w[8];
-                    unpack8<kBF16>(xr[u], x);
+                    unpack8<kBF16>(xc[u], x);
                     unpack8<kBF16>(w_raw[t], w);
                     float r = 1.f;
                     if (normed) {
@@ -176,14 +192,15 @@ qk_norm_kernel(const __grid_constant__ QkNormParams p) {
                         for (int i = 0; i < 8; ++i) o[i] = normed ? x[i] * r * w[i] : x[i];
                         rotate8<kD, kAdjacent, false>(o, cs, sn, upper);
                     } else {
-                        unpack8<kBF16>(gr[u], o);
+                        unpack8<kBF16>(gc[u], o);
                         rotate8<kD, kAdjacent, true>(o, cs, sn, upper);
                         if (normed) {
                             float dot = 0.f;
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 x[i] *= r;  // n
-                                acc[t][i] = fmaf(o[i], x[i], acc[t][i]);
+                                // (a lane behind the last head holds the values of an earlier one)
+                                acc[t][i] += live ? o[i] * x[i] : 0.f;
                                 o[i] *= w[i];
                                 dot = fmaf(o[i], x[i], dot);
                             }
@@ -192,7 +209,7 @@ qk_norm_kernel(const __grid_constant__ QkNormParams p) {
                             for (int i = 0; i < 8; ++i) o[i] = r * (o[i] - x[i] * dot);
                         }
                     }
-                    if (h < h1) __stcs(reinterpret_cast<uint4*>(yb + h * p.y_s[t][2]), pack8<kBF16>(o));
+                    if (live) __stcs(reinterpret_cast<uint4*>(yb + h * p.y_s[t][2]), pack8<kBF16>(o));
                 }
             }
         }

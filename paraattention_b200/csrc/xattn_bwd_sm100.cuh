@@ -60,6 +60,7 @@ struct XBwdParams {
     XSched sched;
     float* part;      // [slot][A1, A2][D / 4][128 rows][4]
     int* status;
+    int* status_host;
     unsigned long long wait_ns;
 };
 
@@ -176,6 +177,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         if ((sX & 1023u) != 0) {  // (never seen; the swizzled tiles would not be where the descriptors say)
             st = PA_DEV_TIMEOUT_PIPE;
             if (p.status != nullptr) atomicCAS(p.status, 0, st);
+            x_report(p.status_host, st);
         }
         ctl->abort = st;
     }
@@ -641,6 +643,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) x_report(p.status_host, ctl->abort);
     if (warp == kXBwdMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
@@ -648,27 +651,28 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 }
 
 // Adds the partial results of units that several CTAs worked on, in range order: one block per
-// unit, 32 columns and accumulator, one thread per row.
+// cut unit, 8 columns and accumulator, one thread per row.
 template <bool kBF16, int kD, bool kKeys>
 __global__ void __launch_bounds__(128)
 xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, int grid) {
-    const int unit = blockIdx.x, cols0 = blockIdx.y * 32, which = blockIdx.z, r = threadIdx.x;
-    float acc[32];
+    XCut cut;
+    if (!x_cut_unit(p.sched, blockIdx.x, grid, cut)) return;
+    const int unit = cut.unit, cols0 = blockIdx.y * 8, which = blockIdx.z, r = threadIdx.x;
+    float acc[8];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    if (!x_for_parts(p.sched, unit, grid, [&](int, int slot) {
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    x_for_parts(p.sched, cut, [&](int slot) {
             const float4* src = reinterpret_cast<const float4*>(p.part) +
                                 ((static_cast<long long>(slot) * 2 + which) * (kD / 4) + cols0 / 4) * kTileM + r;
 #pragma unroll
-            for (int v = 0; v < 8; ++v) {
+            for (int v = 0; v < 2; ++v) {
                 const float4 x = __ldcg(src + v * kTileM);
                 acc[4 * v] += x.x;
                 acc[4 * v + 1] += x.y;
                 acc[4 * v + 2] += x.z;
                 acc[4 * v + 3] += x.w;
             }
-        }))
-        return;
+        });
     XSeg g;
     g.unit = unit;
     g.t0 = g.t1 = 0;
@@ -677,15 +681,11 @@ xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, int grid) {
     if (row >= (kKeys ? p.skv : p.sq)) return;
     const float factor = which ? 1.0f : p.scale;
     uint16_t* grow = p.g[which] + (u.b * p.g_sb[which] + u.head * p.g_sh[which] + row * p.g_ss[which]) + cols0;
+    uint32_t q[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        uint32_t q[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            q[x] = kBF16 ? pack_bf16x2(acc[v * 8 + 2 * x] * factor, acc[v * 8 + 2 * x + 1] * factor)
-                         : pack_f16x2(acc[v * 8 + 2 * x] * factor, acc[v * 8 + 2 * x + 1] * factor);
-        *reinterpret_cast<uint4*>(grow + v * 8) = make_uint4(q[0], q[1], q[2], q[3]);
-    }
+    for (int x = 0; x < 4; ++x)
+        q[x] = kBF16 ? pack_bf16x2(acc[2 * x] * factor, acc[2 * x + 1] * factor) : pack_f16x2(acc[2 * x] * factor, acc[2 * x + 1] * factor);
+    *reinterpret_cast<uint4*>(grow) = make_uint4(q[0], q[1], q[2], q[3]);
 }
 
 // stats[b][h][tile][0 / 1][128] = -lse * log2 e and -sum_d do * out of the query rows; (-inf, 0) for rows without
@@ -703,39 +703,48 @@ __global__ void __launch_bounds__(kXStatThreads)
 xattn_stat_kernel(const __grid_constant__ XStatParams p) {
     constexpr int kLanes = kD / 8;
     const int at = (threadIdx.x % kLanes) * 8;
+    constexpr int kAtOnce = 4;  // vectors per lane in flight
+    constexpr unsigned kGroups = kXStatThreads / kLanes;
     const unsigned n = static_cast<unsigned>(p.batch) * p.heads * p.padded;  // (the host has checked the range)
-    const unsigned step = gridDim.x * (kXStatThreads / kLanes);
     // (heads innermost: neighbouring lanes read neighbouring heads of [B, S, H, D] memory. The trip count
     // is the same for all lanes of a warp - the shuffles need them all.)
-    for (unsigned base = blockIdx.x * (kXStatThreads / kLanes); base < n; base += step) {
-        const unsigned idx = base + threadIdx.x / kLanes;
-        const unsigned t = idx / static_cast<unsigned>(p.heads);
-        const int h = static_cast<int>(idx - t * p.heads);
-        const int b = static_cast<int>(t / static_cast<unsigned>(p.padded));
-        const int s = static_cast<int>(t) - b * p.padded;
-        const bool live = idx < n && s < p.sq;
-        float dot = 0.f;
-        if (live) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.o + (b * p.o_s[0] + h * p.o_s[1] + s * p.o_s[2]) + at));
-            const uint4 y = __ldg(reinterpret_cast<const uint4*>(p.g + (b * p.g_s[0] + h * p.g_s[1] + s * p.g_s[2]) + at));
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    for (unsigned base = blockIdx.x * (kGroups * kAtOnce); base < n; base += gridDim.x * (kGroups * kAtOnce)) {
+        uint4 x[kAtOnce], y[kAtOnce];
+        float l[kAtOnce];
+        unsigned to[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const unsigned idx = base + u * kGroups + threadIdx.x / kLanes;
+            const unsigned t = idx / static_cast<unsigned>(p.heads);
+            const int h = static_cast<int>(idx - t * p.heads);
+            const int b = static_cast<int>(t / static_cast<unsigned>(p.padded));
+            const int s = static_cast<int>(t) - b * p.padded;
+            x[u] = y[u] = make_uint4(0, 0, 0, 0);
+            l[u] = -INFINITY;  // (behind the last query, as without any key)
+            to[u] = idx < n ? (static_cast<unsigned>(b) * p.heads + h) * p.padded + s : ~0u;
+            if (idx < n && s < p.sq) {
+                x[u] = __ldg(reinterpret_cast<const uint4*>(p.o + (b * p.o_s[0] + h * p.o_s[1] + s * p.o_s[2]) + at));
+                y[u] = __ldg(reinterpret_cast<const uint4*>(p.g + (b * p.g_s[0] + h * p.g_s[1] + s * p.g_s[2]) + at));
+                l[u] = __ldg(p.lse + (static_cast<long long>(b) * p.heads + h) * p.sq + s);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const uint32_t xs[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, ys[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+            float dot = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 dot = fmaf(lo16<kBF16>(xs[i]), lo16<kBF16>(ys[i]), dot);
                 dot = fmaf(hi16<kBF16>(xs[i]), hi16<kBF16>(ys[i]), dot);
             }
-        }
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (at == 0 && idx < n) {
-            float2 r = make_float2(-INFINITY, 0.f);
-            if (live) {
-                const float l = __ldg(p.lse + (static_cast<long long>(b) * p.heads + h) * p.sq + s);
-                if (l != -INFINITY) r = make_float2(l * -1.4426950408889634f, -dot);
+            for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (at == 0 && to[u] != ~0u) {
+                const bool none = l[u] == -INFINITY;
+                float* dst = p.stats + static_cast<long long>(to[u] / kTileN) * (2 * kTileN) + to[u] % kTileN;
+                dst[0] = none ? -INFINITY : l[u] * -1.4426950408889634f;
+                dst[kTileN] = none ? 0.f : -dot;
             }
-            float* dst = p.stats + (static_cast<long long>(b) * p.heads + h) * p.padded * 2 + (s / kTileN) * (2 * kTileN) + s % kTileN;
-            dst[0] = r.x;
-            dst[kTileN] = r.y;
         }
     }
 }

@@ -21,6 +21,7 @@
 
 #include "fbc_sm100.cuh"
 #include "pa_ptx.cuh"
+#include "xattn_sm100.cuh"
 
 namespace pa {
 
@@ -40,6 +41,7 @@ struct XFewParams {
     int hkv, group, sq, skv;
     float scale, scale_log2;
     int* status;
+    int* status_host;
     unsigned long long wait_ns;
 };
 
@@ -254,6 +256,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
         if (lane == 0) mbar_arrive(smem_u32(empty + slot));
     }
     __syncthreads();
+    if (threadIdx.x == 0) x_report(p.status_host, *s_abort);
 
     // ---- join the 4 warps: O [warp][16][kD] fp32 over the ring ------------------------------------
     float* wo = reinterpret_cast<float*>(ring);

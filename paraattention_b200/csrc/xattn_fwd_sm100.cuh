@@ -34,6 +34,7 @@ struct XFwdParams {
     float* part_o;    // [slot][D / 4][256 rows][4]
     float2* part_ml;  // [slot][256 rows] (reference, row sum)
     int* status;
+    int* status_host;
     unsigned long long wait_ns;
 };
 
@@ -468,29 +469,29 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) x_report(p.status_host, ctl->abort);
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
 }
 
-// Joins the partial results of units that several CTAs worked on (see XSched): one block per unit
-// and 32 output columns, one thread per row.
+// Joins the partial results of units that several CTAs worked on (see XSched): one block per
+// cut unit and 8 output columns, one thread per row.
 //   out = sum_i 2^((m_i - m) sl) O_i / sum_i 2^((m_i - m) sl) l_i
 template <bool kBF16, int kD>
 __global__ void __launch_bounds__(256)
 xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, int grid) {
-    const int unit = blockIdx.x, cols0 = blockIdx.y * 32, r256 = threadIdx.x;
+    XCut cut;
+    if (!x_cut_unit(p.sched, blockIdx.x, grid, cut)) return;
+    const int unit = cut.unit, cols0 = blockIdx.y * 8, r256 = threadIdx.x;
     const float sl = p.scale_log2;
     float m = -INFINITY;
-    if (!x_for_parts(p.sched, unit, grid, [&](int, int slot) {
-            m = fmaxf(m, __ldcg(p.part_ml + static_cast<long long>(slot) * 256 + r256).x);
-        }))
-        return;
-    float acc[32], l = 0.f;
+    x_for_parts(p.sched, cut, [&](int slot) { m = fmaxf(m, __ldcg(p.part_ml + static_cast<long long>(slot) * 256 + r256).x); });
+    float acc[8], l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    x_for_parts(p.sched, unit, grid, [&](int, int slot) {
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    x_for_parts(p.sched, cut, [&](int slot) {
         const float2 ml = __ldcg(p.part_ml + static_cast<long long>(slot) * 256 + r256);
         if (ml.x == -INFINITY) return;  // (a share that saw no key)
         const float wgt = exp2f((ml.x - m) * sl);
@@ -498,7 +499,7 @@ xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, int grid) {
         const float4* src = reinterpret_cast<const float4*>(p.part_o) +
                             (static_cast<long long>(slot) * (kD / 4) + cols0 / 4) * 256 + r256;
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {
+        for (int v = 0; v < 2; ++v) {
             const float4 x = __ldcg(src + v * 256);
             acc[4 * v] = fmaf(x.x, wgt, acc[4 * v]);
             acc[4 * v + 1] = fmaf(x.y, wgt, acc[4 * v + 1]);
@@ -516,15 +517,11 @@ xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, int grid) {
     const int head = w.hk * p.group + grp;
     const float inv = l > 0.f ? 1.f / l : 0.f;
     uint16_t* orow = p.out + (w.b * p.o_sb + head * p.o_sh + row * p.o_ss) + cols0;
+    uint32_t q[4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        uint32_t q[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            q[x] = kBF16 ? pack_bf16x2(acc[v * 8 + 2 * x] * inv, acc[v * 8 + 2 * x + 1] * inv)
-                         : pack_f16x2(acc[v * 8 + 2 * x] * inv, acc[v * 8 + 2 * x + 1] * inv);
-        *reinterpret_cast<uint4*>(orow + v * 8) = make_uint4(q[0], q[1], q[2], q[3]);
-    }
+    for (int x = 0; x < 4; ++x)
+        q[x] = kBF16 ? pack_bf16x2(acc[2 * x] * inv, acc[2 * x + 1] * inv) : pack_f16x2(acc[2 * x] * inv, acc[2 * x + 1] * inv);
+    *reinterpret_cast<uint4*>(orow) = make_uint4(q[0], q[1], q[2], q[3]);
     if (blockIdx.y == 0 && p.lse != nullptr)
         p.lse[(static_cast<long long>(w.b) * p.hkv * p.group + head) * p.sq + row] =
             l > 0.f ? m * p.scale + logf(l) : -INFINITY;

@@ -19,9 +19,15 @@ namespace pa {
 // has a part of it, and a second launch adds them in range order (results do not depend on
 // scheduling). A CTA has at most one segment that begins inside a unit (slot 2 * CTA) and one
 // that begins with its unit but ends inside it (slot 2 * CTA + 1).
+//
+// Teams (split only): where `team` consecutive units walk the same streamed tiles - the key tiles of one
+// head in the backward kernel's key pass - a team of that many CTAs takes one unit each and one range
+// of steps together, so that a streamed tile comes from HBM once and from L2 for the others. (Single
+// ranges drift apart by a few tiles per CTA: 16380 x 512 x 40 heads read 982 MB from HBM, teams
+// close to the 335 MB that q and do are.)
 struct XSched {
-    int units, steps, split;
-    long long total;  // units * steps
+    int units, steps, split, team;
+    long long total;  // units / team * steps
 };
 
 struct XSeg {
@@ -29,14 +35,15 @@ struct XSeg {
     int slot;  // -1: the whole unit is mine
 };
 
-__host__ __device__ inline long long x_range_begin(const XSched& s, int cta, int grid) {
-    return s.total * cta / grid;
+// First step of a team's range (team = 1: a CTA's), `teams` of them in all.
+__host__ __device__ inline long long x_range_begin(const XSched& s, int index, int teams) {
+    return s.total * index / teams;
 }
-// The CTA whose range holds step `pos`.
-__host__ __device__ inline int x_cta_of(const XSched& s, long long pos, int grid) {
-    int c = static_cast<int>(pos * grid / s.total);
-    while (c > 0 && x_range_begin(s, c, grid) > pos) --c;
-    while (c + 1 < grid && x_range_begin(s, c + 1, grid) <= pos) ++c;
+// The team whose range holds step `pos`.
+__host__ __device__ inline int x_team_of(const XSched& s, long long pos, int teams) {
+    int c = static_cast<int>(pos * teams / s.total);
+    while (c > 0 && x_range_begin(s, c, teams) > pos) --c;
+    while (c + 1 < teams && x_range_begin(s, c + 1, teams) <= pos) ++c;
     return c;
 }
 
@@ -44,8 +51,9 @@ struct XCursor {
     long long pos, end;
     __device__ __forceinline__ explicit XCursor(const XSched& s) {
         if (s.split) {
-            pos = x_range_begin(s, blockIdx.x, gridDim.x);
-            end = x_range_begin(s, blockIdx.x + 1, gridDim.x);
+            const int mine = blockIdx.x / s.team, teams = gridDim.x / s.team;
+            pos = x_range_begin(s, mine, teams);
+            end = x_range_begin(s, mine + 1, teams);
         } else {
             pos = blockIdx.x;
             end = s.units;
@@ -61,8 +69,9 @@ struct XCursor {
             pos += gridDim.x;
             return true;
         }
-        g.unit = static_cast<int>(pos / s.steps);
-        g.t0 = static_cast<int>(pos - static_cast<long long>(g.unit) * s.steps);
+        const int row = static_cast<int>(pos / s.steps);
+        g.unit = row * s.team + blockIdx.x % s.team;
+        g.t0 = static_cast<int>(pos - static_cast<long long>(row) * s.steps);
         const long long left = end - pos;
         g.t1 = left < s.steps - g.t0 ? g.t0 + static_cast<int>(left) : s.steps;
         g.slot = (g.t0 == 0 && g.t1 == s.steps) ? -1 : 2 * static_cast<int>(blockIdx.x) + (g.t0 > 0 ? 0 : 1);
@@ -71,20 +80,36 @@ struct XCursor {
     }
 };
 
-// Calls f(cta, slot) for the CTAs that hold a part of `unit`, in range order; false if one CTA
-// has all of it (then the result is already final).
-template <typename F>
-__device__ __forceinline__ bool x_for_parts(const XSched& s, int unit, int grid, F f) {
-    const long long a = static_cast<long long>(unit) * s.steps, b = a + s.steps;
-    int c = x_cta_of(s, a, grid);
-    if (x_range_begin(s, c + 1, grid) >= b) return false;
-    for (; c < grid; ++c) {
-        const long long r0 = x_range_begin(s, c, grid);
-        if (r0 >= b) break;
-        if (x_range_begin(s, c + 1, grid) == r0) continue;  // (an empty range)
-        f(c, 2 * c + (r0 > a ? 0 : 1));
-    }
+// The units that have to be joined are those that a range begins inside of; a joining launch has (teams - 1) *
+// team blocks, one for each such beginning, of which the first one inside a unit does the work.
+// x_cut_unit: the unit of block `index`, or -1; x_for_parts: calls f(slot) for its parts in range order.
+// (No range is empty: the grid has at most as many teams as there are steps.)
+struct XCut {
+    int unit, first, last;  // teams that have a part of it
+};
+__device__ __forceinline__ bool x_cut_unit(const XSched& s, int index, int grid, XCut& cut) {
+    const int teams = grid / s.team, c = 1 + index / s.team;
+    const long long pos = x_range_begin(s, c, teams), row = pos / s.steps, a = row * s.steps;
+    if (pos == a || x_range_begin(s, c - 1, teams) > a) return false;
+    cut.unit = static_cast<int>(row) * s.team + index % s.team;
+    cut.first = c - 1;
+    cut.last = x_team_of(s, a + s.steps - 1, teams);
     return true;
+}
+template <typename F>
+__device__ __forceinline__ void x_for_parts(const XSched& s, const XCut& cut, F f) {
+    const int member = cut.unit % s.team;
+#pragma unroll 4
+    for (int c = cut.first; c <= cut.last; ++c) f(2 * (c * s.team + member) + (c == cut.first ? 1 : 0));
+}
+
+// A launch in which a wait gave up tells the host, too (one thread of each CTA, at its end): the word is
+// in host memory, so nobody has to copy the device's after every launch.
+__device__ __forceinline__ void x_report(int* status_host, int code) {
+    if (status_host != nullptr && code != 0) {
+        *reinterpret_cast<volatile int*>(status_host) = code;
+        __threadfence_system();
+    }
 }
 
 // ---- key mask -------------------------------------------------------------------------------
