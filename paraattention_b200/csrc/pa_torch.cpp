@@ -263,17 +263,19 @@ pa_qk_norm_args norm_args(const variable_list& xs, const variable_list& ys, cons
 variable_list norm_forward(const variable_list& xs_, const variable_list& ws_, const Tensor& cos, const Tensor& sin,
                            const NormPlan& plan) {
     c10::cuda::CUDAGuard guard(xs_[0].device());
-    variable_list xs, ys, ws;
+    variable_list xs, ys, ws, all;
     for (size_t i = 0; i < xs_.size(); ++i) {
-        ys.push_back(bshd(xs_[i]));
+        all.push_back(bshd(xs_[i]));
+        if (xs_[i].numel() == 0) continue;
+        ys.push_back(all.back());
         xs.push_back(ready(xs_[i]));
         ws.push_back(aligned(ws_[i]));
     }
-    if (xs_[0].numel() == 0) return ys;
+    if (xs.empty()) return all;
     const Tensor c = aligned(cos), s = aligned(sin);
     pa_qk_norm_args a = norm_args(xs, ys, ws, c, s, plan);
     check(pa_qk_norm_fwd(&a, stream_of(xs[0])), false);
-    return ys;
+    return all;
 }
 
 struct QkNorm : public torch::autograd::Function<QkNorm> {
@@ -317,7 +319,7 @@ struct QkNorm : public torch::autograd::Function<QkNorm> {
                 if (!x.defined() || !(asked[i] || asked[i + 2])) continue;
                 const bool weighted = saved[i + 2].defined() && asked[i + 2];
                 const Tensor dy = static_cast<size_t>(i) < grads.size() ? grads[i] : Tensor();
-                if (!dy.defined()) {  // an output nothing depends on
+                if (!dy.defined() || x.numel() == 0) {  // an output nothing depends on, or without elements
                     if (asked[i]) result[i] = at::zeros_like(x);
                     if (weighted) result[i + 2] = at::zeros_like(saved[i + 2]);
                     continue;
@@ -332,27 +334,22 @@ struct QkNorm : public torch::autograd::Function<QkNorm> {
             if (!xs.empty()) {
                 bool any_weight = false;
                 for (const Tensor& w : dws) any_weight = any_weight || w.defined();
-                if (xs[0].numel() == 0) {
-                    for (Tensor& w : dws)
-                        if (w.defined()) w.zero_();
-                } else {
-                    const Tensor cos = aligned(saved[4]), sin = aligned(saved[5]);
-                    pa_qk_norm_args a = norm_args(xs, dxs, ws, cos, sin, plan);
-                    for (size_t i = 0; i < xs.size(); ++i) {
-                        a.dy[i] = dys[i].data_ptr();
-                        int64_t s[3];
-                        strides(dys[i], s);
-                        a.dy_stride[i][0] = s[0], a.dy_stride[i][1] = s[2], a.dy_stride[i][2] = s[1];
-                        if (dws[i].defined()) a.dweight[i] = dws[i].data_ptr();
-                    }
-                    Tensor scratch;
-                    if (any_weight) {
-                        scratch = at::empty({pa_qk_norm_workspace_bytes()}, xs[0].options().dtype(at::kByte));
-                        a.workspace = scratch.data_ptr();
-                        a.workspace_bytes = scratch.numel();
-                    }
-                    check(pa_qk_norm_bwd(&a, stream_of(xs[0])), true);
+                const Tensor cos = aligned(saved[4]), sin = aligned(saved[5]);
+                pa_qk_norm_args a = norm_args(xs, dxs, ws, cos, sin, plan);
+                for (size_t i = 0; i < xs.size(); ++i) {
+                    a.dy[i] = dys[i].data_ptr();
+                    int64_t s[3];
+                    strides(dys[i], s);
+                    a.dy_stride[i][0] = s[0], a.dy_stride[i][1] = s[2], a.dy_stride[i][2] = s[1];
+                    if (dws[i].defined()) a.dweight[i] = dws[i].data_ptr();
                 }
+                Tensor scratch;
+                if (any_weight) {
+                    scratch = at::empty({pa_qk_norm_workspace_bytes()}, xs[0].options().dtype(at::kByte));
+                    a.workspace = scratch.data_ptr();
+                    a.workspace_bytes = scratch.numel();
+                }
+                check(pa_qk_norm_bwd(&a, stream_of(xs[0])), true);
                 for (size_t i = 0; i < which.size(); ++i) {
                     if (asked[which[i]]) result[which[i]] = dxs[i];
                     if (dws[i].defined()) result[which[i] + 2] = dws[i];

@@ -366,6 +366,15 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                     uint32_t live = 0xffffffffu;
                     uint32_t pk[16];
                     float ls, mx;
+                    if (c == 0 && i == 0) {
+                        // A row's first logits set its reference: with few key tiles the guess from earlier pieces,
+                        // which the later ones take, would be wrong once in every 16 pieces.
+                        const uint32_t seen = plain ? 0xffffffffu : static_cast<uint32_t>(kw0);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2)
+                            m_ref = fmax3(m_ref, ((seen >> x) & 1u) ? __uint_as_float(sc[x]) : -INFINITY,
+                                          ((seen >> (x + 1)) & 1u) ? __uint_as_float(sc[x + 1]) : -INFINITY);
+                    }
                     const float neg = (m_ref == -INFINITY) ? 0.0f : -m_ref * sl;
                     if (plain) {
                         softmax_chunk<kBF16, false>(sc, live, sl, neg, pk, ls, mx);

@@ -333,6 +333,34 @@ def test_calls_at_once_on_two_streams():
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("Sq", [3, 200])
+def test_rows_more_than_four_gigabytes_apart(Sq):
+    """Keys, values and queries as views with a row step of 2 MB over a buffer of 5 GB: offsets pass 32 bits."""
+    B, H, Skv, D, step = 1, 1, 2400, 64, 1 << 20
+    big = torch.empty(Skv * step, dtype=torch.bfloat16, device="cuda")
+    q, k, v, do = make(B, H, H, Sq, Skv, D)
+    far = lambda at, rows: big.as_strided((B, H, rows, D), (0, 0, step, 1), at)  # noqa: E731
+    kf, vf, qf = far(0, Skv), far(64, Skv), far(128, Sq)
+    for f, x in ((kf, k), (vf, v), (qf, q)):
+        f.copy_(x)
+    leaves = [t.requires_grad_(True) for t in (qf, kf, vf)]
+    want = check_gradients(*leaves, do)
+    near = [t.detach().contiguous().requires_grad_(True) for t in leaves]
+    out = ops.cross_attention(*near)
+    assert torch.equal(out, want[0])
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, near, do), want[1:]))
+    assert torch.equal(ops.cross_attention(*(t.detach() for t in leaves)), want[0])
+
+
+@pytest.mark.parametrize("size", [(1, 200, 1, 1, 40), (300, 2, 2, 1, 9), (40, 3, 3, 18, 5), (2, 16, 1, 1, 70), (2, 17, 1, 1, 70)])
+def test_many_units_of_few_rows(size):
+    """Many heads or sequences with hardly any rows: both sides of the limit of 16 rows per key head."""
+    q, k, v, do = make(*size, 64, grad=True)
+    check_gradients(q, k, v, do)
+    with torch.no_grad():
+        check_forward(q, k, v)
+
+
 def test_what_lies_behind_the_tensors_is_left_alone():
     """Rows of a larger buffer behind the last key and query are neither read nor written."""
     B, H, Sq, Skv, D = 1, 2, 37, 45, 64

@@ -113,6 +113,23 @@ def test_strides_alignment_and_zero_rows():
     g, = torch.autograd.grad(y, z, torch.ones_like(y))
     assert not y.any() and bool(g.isfinite().all())
     assert ops.qk_norm_rotary(q[:, :, :0], k[:, :, :0], wq, wk, rotary)[0].shape == (B, H, 0, D)
+    none, some = ops.qk_norm_rotary(q[:, :0], k, wq, wk, rotary)
+    assert none.shape == (B, 0, S, D) and torch.equal(some, want[1])
+    leaves = [t.detach().requires_grad_(True) for t in (q[:, :0], k, wq, wk)]
+    y = ops.qk_norm_rotary(*leaves, rotary)
+    grads = torch.autograd.grad(y, leaves, [torch.ones_like(t) for t in y])
+    assert grads[0].numel() == 0 and not grads[2].any() and bool(grads[3].any())
+
+
+def test_rows_more_than_four_gigabytes_apart():
+    step, S, D = 1 << 20, 2400, 64
+    big = torch.empty(S * step, dtype=torch.bfloat16, device="cuda")
+    q, _, wq, _, rotary, dq, _ = make(1, 1, 1, S, D, torch.bfloat16)
+    far = big.as_strided((1, 1, S, D), (0, 0, step, 1)).copy_(q).requires_grad_(True)
+    near = q.detach().requires_grad_(True)
+    a, b = (ops.qk_norm_rotary(t, None, wq, None, rotary)[0] for t in (far, near))
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, far, dq)[0], torch.autograd.grad(b, near, dq)[0])
 
 
 def test_repeats_streams_and_graphs_give_the_same_bits():
