@@ -134,7 +134,7 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     auto kern = pa::xattn_fwd_kernel<kBF16, kD>;
     rc = allow_smem(kern, pa::kXFwdSmemBytes, "xattn forward");
     if (rc != PA_OK) return rc;
-    kern<<<f.grid, pa::kAttnThreads, pa::kXFwdSmemBytes, s>>>(mq, mk, mv, mo, p);
+    kern<<<f.grid, pa::kXFwdThreads, pa::kXFwdSmemBytes, s>>>(mq, mk, mv, mo, p);
     rc = launched("xattn forward");
     if (rc != PA_OK || !f.sched.split || f.grid == f.sched.team) return rc;
     pa::xattn_fwd_join_kernel<kBF16, kD><<<dim3(f.grid - f.sched.team, kD / 8), 256, 0, s>>>(p, f.grid);

@@ -87,7 +87,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
     constexpr int kRowBytes = kD * 2;
     constexpr int kTile = kFewKeys * kRowBytes;     // bytes of a K or V tile
     constexpr int kStage = 2 * kTile;               // K, V
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sq_ = smem;
     uint8_t* ring = smem + kFewRows * kRowBytes;
     float2* wml = reinterpret_cast<float2*>(ring + kFewStages * kStage);  // [4 warps][16 rows]

@@ -10,10 +10,19 @@
 //
 // A unit is two row tiles of 128 queries that share a key / value head: tile i of (batch, kv head)
 // is query head i / mt, rows (i % mt) * 128, mt = ceil(Sq / 128) - so with short queries two heads
-// of a group share one pass over the keys. Inside a unit the pipeline is that of the long kernel
-// (half tiles in the key dimension, one-pass softmax in pieces of 32 columns, lazily rescaled O).
-// Warps: 0-7 softmax (one thread per query row), 8 MMA issuer, 9 TMA producer, 10 clears masked
-// rows of V (only with a mask). TMEM columns: S0 S1 [0,256), O0 O1 [256, 256 + 2 D).
+// of a group share one pass over the keys. The two tiles take turns: while one is in its softmax the
+// tensor core runs the other's P V and next Q K^T.
+//
+// Two threads share a row, 64 key columns each (16 softmax warps). That halves the softmax's latency,
+// which is what lets Q K^T run on whole tiles: the long kernel's one thread per row is too slow for that
+// and splits Q K^T into N = 64 halves, which cost 66 cycles of shared-memory operand fetch each instead of
+// 32 (3136 cycles of products per key tile and unit instead of 2048). The threads of a row meet once per
+// key tile, to agree on its maximum; O is rescaled lazily, when a row outgrows the reference its weights
+// are relative to by more than 2^8.
+//
+// Warps: 0-15 softmax and epilogue (tile w / 8, columns half (w / 4) % 2, TMEM lane quarter w % 4), 16 MMA
+// issuer, 17 TMA producer, 18 clears masked rows of V (only with a mask). TMEM columns: S0 S1 [0,256),
+// O0 O1 [256, 256 + 2 D); P overwrites S.
 //
 // Bounds: bytes q, k, v read + out written once at HBM rate, or 4 Sq Skv D flops per head at the
 // tensor rate. A unit re-reads its head's K and V from L2.
@@ -21,6 +30,10 @@
 #include "xattn_sm100.cuh"
 
 namespace pa {
+
+constexpr int kXFwdSoftWarps = 16;
+constexpr int kXFwdMmaWarp = 16, kXFwdTmaWarp = 17, kXFwdCleanWarp = 18;
+constexpr int kXFwdThreads = 640;
 
 struct XFwdParams {
     int batch, kv_batch, hkv, group, sq, skv, mt;
@@ -41,17 +54,18 @@ struct XFwdParams {
 struct XFwdCtl {
     uint64_t q_full, q_empty;
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2];
-    uint64_t s_full[2][2];
-    uint64_t p_full[2][kPieces];
-    uint64_t o_done[2][kPieces];
+    uint64_t s_full[2];     // Q K^T of a row tile is in TMEM
+    uint64_t p_full[2];     // P of a row tile is in TMEM and its O is rescaled (one arrival per warp)
+    uint64_t o_done[2];     // P V of a row tile (and every product before it) is done
     uint64_t teardown;
     uint32_t tmem_base;
     int abort;
 };
-// alignment slack; Q, K and V ring; output staging, two buffers for each softmax warp; control block
-constexpr int kXFwdSmemBytes = 1024 + 6 * kTileBytes + 2 * kSoftmaxWarps * kXStageBytes + 512;
-static_assert(kXFwdSmemBytes <= 232448, "shared memory");
+// Q, K and V ring; output staging, one buffer for each softmax warp; what the two threads of a row exchange; control
+// block. (The dynamic shared memory is declared with the alignment of the swizzle; there is no room for slack.)
+constexpr int kXFwdSmemBytes = 6 * kTileBytes + kXFwdSoftWarps * kXStageBytes + kXFwdSoftWarps * 32 * 4 + 512;
 static_assert(sizeof(XFwdCtl) <= 512, "control block too large");
+static_assert(kXFwdSmemBytes <= 232448, "shared memory");
 
 // What a segment of work means: which rows, which keys.
 struct XFwdUnit {
@@ -77,23 +91,30 @@ __device__ __forceinline__ XFwdUnit x_fwd_unit(const XFwdParams& p, const XSeg& 
 }
 
 template <bool kBF16, int kD>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kXFwdThreads, 1)
 xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
                  const __grid_constant__ XFwdParams p) {
     constexpr int kAtoms = kD / 64;
     constexpr int kOperandBytes = kAtoms * kHalfBytes;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw_addr = smem_u32(smem_raw);
-    uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+    extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sQ = smem_u32(smem);
     const uint32_t sK = sQ + 2 * kTileBytes;
     const uint32_t sV = sK + 2 * kTileBytes;
-    XFwdCtl* ctl = reinterpret_cast<XFwdCtl*>(smem + 6 * kTileBytes + 2 * kSoftmaxWarps * kXStageBytes);
+    float* exchange = reinterpret_cast<float*>(smem + 6 * kTileBytes + kXFwdSoftWarps * kXStageBytes);  // [warp][32]
+    XFwdCtl* ctl = reinterpret_cast<XFwdCtl*>(exchange + kXFwdSoftWarps * 32);
     volatile int* s_abort = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (threadIdx.x == 0) ctl->abort = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+    if (threadIdx.x == 0) {
+        int st = p.status != nullptr ? *reinterpret_cast<volatile int*>(p.status) : 0;
+        if ((sQ & 1023u) != 0) {  // (never seen; the swizzled tiles would not be where the descriptors say)
+            st = PA_DEV_TIMEOUT_PIPE;
+            if (p.status != nullptr) atomicCAS(p.status, 0, st);
+            x_report(p.status_host, st);
+        }
+        ctl->abort = st;
+    }
     __syncthreads();
     if (ctl->abort != 0) return;
     if (threadIdx.x == 0) {
@@ -105,21 +126,18 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             mbar_init(smem_u32(&ctl->v_full[s]), 1);
             mbar_init(smem_u32(&ctl->v_empty[s]), 1);
             mbar_init(smem_u32(&ctl->v_clean[s]), 1);
-            mbar_init(smem_u32(&ctl->s_full[s][0]), 1);
-            mbar_init(smem_u32(&ctl->s_full[s][1]), 1);
-            for (int c = 0; c < kPieces; ++c) {
-                mbar_init(smem_u32(&ctl->p_full[s][c]), kTileM);
-                mbar_init(smem_u32(&ctl->o_done[s][c]), 1);
-            }
+            mbar_init(smem_u32(&ctl->s_full[s]), 1);
+            mbar_init(smem_u32(&ctl->p_full[s]), 8);
+            mbar_init(smem_u32(&ctl->o_done[s]), 1);
         }
         mbar_init(smem_u32(&ctl->teardown), 1);
         mbar_init_fence();
     }
-    if (warp == kMmaWarp) {
+    if (warp == kXFwdMmaWarp) {
         tmem_alloc(smem_u32(&ctl->tmem_base), kTmemCols);
         tmem_relinquish();
     }
-    if (warp == kTmaWarp && lane == 0) {
+    if (warp == kXFwdTmaWarp && lane == 0) {
         tma_prefetch_desc(&tm_q);
         tma_prefetch_desc(&tm_k);
         tma_prefetch_desc(&tm_v);
@@ -134,7 +152,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
     XCursor cursor(p.sched);
     XSeg seg;
-    if (warp == kTmaWarp) {
+    if (warp == kXFwdTmaWarp) {
         // =============================== TMA producer ======================================
         if (lane == 0) {
             bool ok = true;
@@ -190,9 +208,9 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 }
             }
         }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == kXFwdMmaWarp) {
         // =============================== MMA issuer ========================================
-        constexpr uint32_t idesc_qk = make_idesc_f16(kBF16, false, kTileM, kTileN / 2);
+        constexpr uint32_t idesc_qk = make_idesc_f16(kBF16, false, kTileM, kTileN);
         constexpr uint32_t idesc_pv = make_idesc_f16(kBF16, true, kTileM, kD);
         const uint32_t leader = elect_one() ? 1u : 0u;
         const uint64_t dq0 = smem_desc_sw128(sQ, 16, 1024);
@@ -200,26 +218,25 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         const uint32_t hi_qk = static_cast<uint32_t>(dq0 >> 32), hi_v = static_cast<uint32_t>(dv0 >> 32);
         const uint32_t lo_q = static_cast<uint32_t>(dq0), lo_v = static_cast<uint32_t>(dv0);
         const uint32_t lo_k = static_cast<uint32_t>(smem_desc_sw128(sK, 16, 1024));
-        auto issue_qk_half = [&](int t, int st, int half) {
-            const uint32_t a0 = lo_q + ((t * kTileBytes) >> 4);
-            const uint32_t b0 = lo_k + ((st * kTileBytes + half * 64 * 128) >> 4);
-            const uint32_t d = tmem + kColS0 + t * kTileN + half * (kTileN / 2);
+        auto issue_qk = [&](int t, int st) {
+            const uint32_t a0 = lo_q + ((t * kTileBytes) >> 4), b0 = lo_k + ((st * kTileBytes) >> 4);
+            const uint32_t d = tmem + kColS0 + t * kTileN;
 #pragma unroll
             for (int ks = 0; ks < kD / 16; ++ks) {
                 const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
                 tc_mma_ss_elect(d, a0 + off, hi_qk, b0 + off, hi_qk, idesc_qk, ks > 0 ? 1u : 0u, leader);
             }
+            tc_commit_elect(smem_u32(&ctl->s_full[t]), leader);
         };
-        auto issue_pv_piece = [&](int t, int st, int piece, bool acc) {
+        // 16 keys a k-step; their P is 8 packed columns (32 columns of S are packed into their first 16)
+        auto issue_pv = [&](int t, int st, bool acc) {
             const uint32_t b0 = lo_v + ((st * kTileBytes) >> 4);
             const uint32_t a0 = tmem + kColS0 + t * kTileN;
-            const uint32_t d = tmem + kColO0 + t * kD;
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-                const int ks = piece * 2 + k2;
-                tc_mma_ts_elect(d, a0 + (piece >> 1) * (kTileN / 2) + (ks & 3) * 8, b0 + ((ks * 16 * 128) >> 4), hi_v,
+            for (int ks = 0; ks < 8; ++ks)
+                tc_mma_ts_elect(tmem + kColO0 + t * kD, a0 + (ks >> 1) * 32 + (ks & 1) * 8, b0 + ((ks * 16 * 128) >> 4), hi_v,
                                 idesc_pv, (acc || ks > 0) ? 1u : 0u, leader);
-            }
+            tc_commit_elect(smem_u32(&ctl->o_done[t]), leader);
         };
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
             const bool r = mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE);
@@ -235,13 +252,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             if (!ok) break;
             tc_fence_after();
             issued = true;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    issue_qk_half(t, j & 1, half);
-                    tc_commit_elect(smem_u32(&ctl->s_full[t][half]), leader);
-                }
+            issue_qk(0, j & 1);
+            issue_qk(1, j & 1);
             tc_commit_elect(smem_u32(&ctl->k_empty[j & 1]), leader);
             if (n == 1) tc_commit_elect(smem_u32(&ctl->q_empty), leader);
             for (int i = 0; i < n && ok; ++i, ++j) {
@@ -251,29 +263,19 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 if (ok && more) ok = wait(&ctl->k_full[stn], ((j + 1) >> 1) & 1);
                 if (!ok) break;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                        for (int c = 2 * half; c < 2 * half + 2; ++c) {
-                            ok = wait(&ctl->p_full[t][c], j & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            issue_pv_piece(t, st, c, i > 0);
-                            tc_commit_elect(smem_u32(&ctl->o_done[t][c]), leader);
-                        }
-                        if (!ok) break;
-                        if (half == 1 && t == 1) tc_commit_elect(smem_u32(&ctl->v_empty[st]), leader);
-                        if (more) {
-                            issue_qk_half(t, stn, half);
-                            tc_commit_elect(smem_u32(&ctl->s_full[t][half]), leader);
-                            if (half == 1 && t == 1) {
-                                tc_commit_elect(smem_u32(&ctl->k_empty[stn]), leader);
-                                if (i + 2 == n) tc_commit_elect(smem_u32(&ctl->q_empty), leader);
-                            }
+                for (int t = 0; t < 2; ++t) {
+                    ok = wait(&ctl->p_full[t], j & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(t, st, i > 0);
+                    if (t == 1) tc_commit_elect(smem_u32(&ctl->v_empty[st]), leader);
+                    if (more) {
+                        issue_qk(t, stn);
+                        if (t == 1) {
+                            tc_commit_elect(smem_u32(&ctl->k_empty[stn]), leader);
+                            if (i + 2 == n) tc_commit_elect(smem_u32(&ctl->q_empty), leader);
                         }
                     }
-                    if (!ok) break;
                 }
             }
             ++u;
@@ -285,7 +287,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             tc_commit_elect(smem_u32(&ctl->teardown), leader);
             mbar_wait(smem_u32(&ctl->teardown), 0, no_abort, nullptr, 100000000ull, 0);
         }
-    } else if (warp == kTmaWarp + 1 && p.words != nullptr) {
+    } else if (warp == kXFwdCleanWarp && p.words != nullptr) {
         // =============================== masked rows of V ==================================
         bool ok = true;
         int j = 0;
@@ -308,178 +310,163 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
                 if (lane == 0) mbar_arrive(smem_u32(&ctl->v_clean[st]));
             }
         }
-    } else if (warp < kSoftmaxWarps) {
+    } else if (warp < kXFwdSoftWarps) {
         // =============================== softmax + epilogue ================================
-        const int quarter = warp & 3, t = warp >> 2;
+        // (Nobody leaves this loop early: the two warps of a row meet at named barriers, which both must reach the
+        // same number of times. Once the abort word is set no wait blocks any more.)
+        const int t = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
         const int row_in_tile = quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t tS = tmem + lane_base + kColS0 + t * kTileN;
-        const uint32_t tO = tmem + lane_base + kColO0 + t * kD;
+        const uint32_t tS = tmem + lane_base + kColS0 + t * kTileN + half * 64;      // my 64 logits
+        const uint32_t tO = tmem + lane_base + kColO0 + t * kD + half * (kD / 2);    // my half of the row's output
+        float* mine = exchange + warp * 32 + lane;
+        const float* other = exchange + (warp ^ 4) * 32 + lane;
+        uint8_t* stage = smem + 6 * kTileBytes + warp * kXStageBytes;
         const float sl = p.scale_log2;
-        bool ok = true;
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + quarter) : "memory"); };
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, s_abort, p.status, limit, PA_DEV_TIMEOUT_PIPE));
+        };
         int j = 0;
-        while (ok && cursor.next(p.sched, seg)) {
+        while (cursor.next(p.sched, seg)) {
             const XFwdUnit w = x_fwd_unit(p, seg);
             const int n = w.hi - w.lo;
             const unsigned long long* mrow = p.words != nullptr ? p.words + static_cast<long long>(w.b) * n_words : nullptr;
             float m_ref = -INFINITY, l_sum = 0.f;
-            uint32_t buf[2][32];
-            bool pre = false;
-            int pending = -1;
-            for (int i = 0; i < n && ok; ++i, ++j) {
-                const unsigned long long kw0 = x_key_word(mrow, p.skv, 2 * (w.lo + i));
-                const unsigned long long kw1 = x_key_word(mrow, p.skv, 2 * (w.lo + i) + 1);
-                const bool plain = (kw0 & kw1) == ~0ull;  // (the same for the whole CTA)
-#pragma unroll
-                for (int c = 0; c < kPieces; ++c) {
-                    const int half = c >> 1, hc = c & 1;
-                    uint32_t(&sc)[32] = buf[hc];
-                    if (!pre) {
-                        if (pending >= 0) {  // never block with a hand-over outstanding
-                            tc_wait_st();
-                            tc_fence_before();
-                            mbar_arrive(smem_u32(&ctl->p_full[t][pending]));
-                            pending = -1;
-                        }
-                        if (hc == 0) {
-                            // (a vote: a wait that gives up in some lanes only must not split the warp)
-                            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ctl->s_full[t][half]), j & 1, s_abort,
-                                                                   p.status, limit, PA_DEV_TIMEOUT_PIPE)) && ok;
-                            tc_fence_after();
-                        }
-                        tmem_ld32(tS + c * kPieceCols, sc);
-                    }
+            for (int i = 0; i < n; ++i, ++j) {
+                const unsigned long long word = x_key_word(mrow, p.skv, 2 * (w.lo + i) + half);
+                const bool plain = word == ~0ull;  // (the same for the whole warp)
+                wait(&ctl->s_full[t], j & 1);
+                tc_fence_after();
+                // Two passes over the logits, 32 at a time, the second in the opposite order: 96 registers do not
+                // hold 64 of them, and reading TMEM again costs less than spilling.
+                uint32_t sc[32];
+                float mx[2] = {-INFINITY, -INFINITY};
+                auto fetch = [&](int c) {
+                    tmem_ld32(tS + c * 32, sc);
                     tc_wait_ld();
                     tmem_ld_fence(sc);
-                    pre = false;
-                    if (hc == 0) {
-                        pre = true;
-                    } else if (c == 1) {
-                        pre = __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&ctl->s_full[t][1]), j & 1));
-                    } else if (i + 1 < n) {
-                        pre = __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&ctl->s_full[t][0]), (j + 1) & 1));
-                    }
-                    if (pre) {
-                        if (hc == 1) tc_fence_after();
-                        tmem_ld32(tS + ((c + 1) & 3) * kPieceCols, buf[hc ^ 1]);
-                    }
-                    uint32_t live = 0xffffffffu;
-                    uint32_t pk[16];
-                    float ls, mx;
-                    if (c == 0 && i == 0) {
-                        // A row's first logits set its reference: with few key tiles the guess from earlier pieces,
-                        // which the later ones take, would be wrong once in every 16 pieces.
-                        const uint32_t seen = plain ? 0xffffffffu : static_cast<uint32_t>(kw0);
+                    if (!plain) {
+                        const uint32_t live = static_cast<uint32_t>(word >> (c * 32));
 #pragma unroll
-                        for (int x = 0; x < 32; x += 2)
-                            m_ref = fmax3(m_ref, ((seen >> x) & 1u) ? __uint_as_float(sc[x]) : -INFINITY,
-                                          ((seen >> (x + 1)) & 1u) ? __uint_as_float(sc[x + 1]) : -INFINITY);
+                        for (int x = 0; x < 32; ++x)
+                            if (((live >> x) & 1u) == 0) sc[x] = __float_as_uint(-INFINITY);
                     }
-                    const float neg = (m_ref == -INFINITY) ? 0.0f : -m_ref * sl;
-                    if (plain) {
-                        softmax_chunk<kBF16, false>(sc, live, sl, neg, pk, ls, mx);
-                    } else {
-                        live = static_cast<uint32_t>((half ? kw1 : kw0) >> (hc * 32));
-                        softmax_chunk<kBF16, true>(sc, live, sl, neg, pk, ls, mx);
-                    }
-                    if (pending >= 0) {
-                        tc_wait_st();
-                        tc_fence_before();
-                        mbar_arrive(smem_u32(&ctl->p_full[t][pending]));
-                        pending = -1;
-                    }
-                    const bool grow = (mx - m_ref) * sl > kRescaleThreshold;  // (-inf - -inf: NaN, false)
-                    const uint32_t tP = tS + half * (kTileN / 2) + hc * (kPieceCols / 2);
-                    if (__any_sync(0xffffffffu, grow)) {
-                        if (pre) {
-                            tc_wait_ld();
-                            tmem_ld_fence(buf[hc ^ 1]);
-                        }
-                        const uint32_t bo = (c > 0) ? smem_u32(&ctl->o_done[t][c - 1]) : smem_u32(&ctl->o_done[t][kPieces - 1]);
-                        const uint32_t par = (c > 0) ? (j & 1) : ((j - 1) & 1);
-                        const float2 r = softmax_piece_regrow<kBF16, kD>(tS + c * kPieceCols, tP, tO, live, sl, mx, m_ref,
-                                                                         l_sum, i > 0 || c > 0, bo, par, s_abort, p.status,
-                                                                         limit);
-                        m_ref = r.x;
-                        l_sum = r.y;
-                    } else {
-                        l_sum += ls;
-                        tmem_st16(tP, pk);
-                    }
-                    if (hc == 0) {
-                        pending = c;
-                    } else {
-                        tc_wait_st();
-                        tc_fence_before();
-                        mbar_arrive(smem_u32(&ctl->p_full[t][c]));
+                };
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    fetch(c);
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        mx[0] = fmax3(mx[0], __uint_as_float(sc[x]), __uint_as_float(sc[x + 1]));
+                        mx[1] = fmax3(mx[1], __uint_as_float(sc[x + 2]), __uint_as_float(sc[x + 3]));
                     }
                 }
+                // The row's maximum. (The buffer needs no second copy: the next logits of this tile are there only
+                // after both threads have handed over their P, that is, after both have read.)
+                const float own = fmaxf(mx[0], mx[1]);
+                *mine = own;
+                meet();
+                const float row_max = fmaxf(own, *other);
+                const bool grow = (row_max - m_ref) * sl > kRescaleThreshold;  // (-inf - -inf: NaN, false)
+                if (__any_sync(0xffffffffu, grow)) {  // (the same in both warps of the rows)
+                    const float m_new = fmaxf(m_ref, row_max);
+                    const float alpha = m_new == -INFINITY ? 1.0f : ex2_approx((m_ref - m_new) * sl);
+                    m_ref = m_new;
+                    l_sum *= alpha;
+                    if (i > 0) {
+                        wait(&ctl->o_done[t], (j - 1) & 1);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int b = 0; b < kD / 64; ++b) {
+                            uint32_t o[32];
+                            tmem_ld32(tO + b * 32, o);
+                            tc_wait_ld();
+                            tmem_ld_fence(o);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+                            tmem_st32(tO + b * 32, o);
+                        }
+                    }
+                }
+                const float neg = m_ref == -INFINITY ? 0.0f : -m_ref * sl;
+                const float2 sl2 = make_float2(sl, sl), neg2 = make_float2(neg, neg);
+                float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 1; c >= 0; --c) {
+                    if (c == 0) fetch(0);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(sc[x]), __uint_as_float(sc[x + 1])), sl2, neg2);
+                        const float2 e = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                        ls[(x >> 1) & 1] = __fadd2_rn(ls[(x >> 1) & 1], e);
+                        pk[x >> 1] = kBF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+                    }
+                    tmem_st16(tS + c * 32, pk);
+                }
+                const float2 sum = __fadd2_rn(ls[0], ls[1]);
+                l_sum += sum.x + sum.y;
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl->p_full[t]));
             }
-            if (n > 0)
-                ok = mbar_wait(smem_u32(&ctl->o_done[t][kPieces - 1]), (j - 1) & 1, s_abort, p.status, limit,
-                               PA_DEV_TIMEOUT_PIPE) && ok;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            // ---- the unit's output: my half of the row's columns -----------------------------------
+            if (n > 0) wait(&ctl->o_done[t], (j - 1) & 1);
             tc_fence_after();
+            *mine = l_sum;
+            meet();
+            l_sum += *other;
             const int tile = w.tile0 + t, g = tile / p.mt;
             const int row = (tile - g * p.mt) * kTileM + row_in_tile;
-            const bool in_range = g < p.group && row < p.sq;
             const int head = w.hk * p.group + g;
-            if (seg.slot >= 0) {
-                // this CTA's share of a unit: unnormalised O, reference and row sum
-                const int r256 = t * kTileM + row_in_tile;
-                float4* po = reinterpret_cast<float4*>(p.part_o) + static_cast<long long>(seg.slot) * (kD / 4) * 256 + r256;
-#pragma unroll
-                for (int b = 0; b < kD / 32; ++b) {
-                    uint32_t o[32];
-                    tmem_ld32(tO + b * 32, o);
-                    tc_wait_ld();
-                    tmem_ld_fence(o);
-                    if (n <= 0) {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) o[x] = 0u;
-                    }
-#pragma unroll
-                    for (int v4 = 0; v4 < 8; ++v4)
-                        __stcg(po + (b * 8 + v4) * 256,
-                               make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
-                                           __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
-                }
-                __stcg(p.part_ml + static_cast<long long>(seg.slot) * 256 + r256, make_float2(m_ref, l_sum));
-                continue;
-            }
-            const float inv = l_sum > 0.0f ? 1.0f / l_sum : 0.0f;  // (no key at all: zeros, LSE -inf)
-            uint8_t* stage = smem + 6 * kTileBytes + warp * (2 * kXStageBytes);
-            const bool zero = n <= 0 || !(l_sum > 0.0f);
+            const bool none = n <= 0 || !(l_sum > 0.0f);  // no key at all: zeros, LSE -inf
+            const float inv = none ? 0.0f : 1.0f / l_sum;
             const int row_w = (tile - g * p.mt) * kTileM + quarter * 32;  // first of the warp's rows
-#pragma unroll
-            for (int b = 0; b < kD / 32; ++b) {
+#pragma unroll 1
+            for (int b = 0; b < kD / 64; ++b) {
                 uint32_t o[32];
                 tmem_ld32(tO + b * 32, o);
-                if (lane == 0) tma_store_wait_read<1>();  // (this buffer's last store has been read)
+                if (seg.slot < 0 && lane == 0) tma_store_wait_read();  // (the staging memory is free again)
                 __syncwarp();
                 tc_wait_ld();
                 tmem_ld_fence(o);
-                if (zero) {
+                if (none) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x) o[x] = 0u;
                 }
-                x_stage32<kBF16>(stage + (b & 1) * kXStageBytes, lane, o, inv);
-                fence_proxy_async_shared();
-                __syncwarp();
-                if (lane == 0 && g < p.group && row_w < p.sq)
-                    tma_store_5d(&tm_o, smem_u32(stage + (b & 1) * kXStageBytes), b * 32, row_w, head, w.b, 0);
+                const int col = half * (kD / 2) + b * 32;
+                if (seg.slot < 0) {
+                    x_stage32<kBF16>(stage, lane, o, inv);
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0 && g < p.group && row_w < p.sq) tma_store_5d(&tm_o, smem_u32(stage), col, row_w, head, w.b, 0);
+                } else {  // this CTA's share of a unit: unnormalised O
+                    float4* po = reinterpret_cast<float4*>(p.part_o) + static_cast<long long>(seg.slot) * (kD / 4) * 256 +
+                                 (col / 4) * 256 + t * kTileM + row_in_tile;
+#pragma unroll
+                    for (int v4 = 0; v4 < 8; ++v4)
+                        __stcg(po + v4 * 256, make_float4(__uint_as_float(o[4 * v4]), __uint_as_float(o[4 * v4 + 1]),
+                                                          __uint_as_float(o[4 * v4 + 2]), __uint_as_float(o[4 * v4 + 3])));
+                }
             }
-            if (in_range && p.lse != nullptr)
-                p.lse[(static_cast<long long>(w.b) * p.hkv * p.group + head) * p.sq + row] =
-                    l_sum > 0.0f ? m_ref * p.scale + logf(l_sum) : -INFINITY;
+            if (half == 0) {
+                if (seg.slot >= 0)
+                    __stcg(p.part_ml + static_cast<long long>(seg.slot) * 256 + t * kTileM + row_in_tile, make_float2(m_ref, l_sum));
+                else if (p.lse != nullptr && g < p.group && row < p.sq)
+                    p.lse[(static_cast<long long>(w.b) * p.hkv * p.group + head) * p.sq + row] =
+                        none ? -INFINITY : m_ref * p.scale + logf(l_sum);
+            }
+            tc_fence_before();
+            meet();  // (both have read the other's sum)
         }
         if (lane == 0) tma_store_wait();
     }
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0) x_report(p.status_host, ctl->abort);
-    if (warp == kMmaWarp) {
+    if (warp == kXFwdMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
