@@ -32,6 +32,28 @@ FwdPlan plan(const pa_xattn_args* a) {
     return f;
 }
 
+// CTAs per (batch, kv head) for `units` of them with `tiles` key tiles each: the least time by a model fitted to
+// measurements (microseconds, head_dim 128; half the bytes at 64): 7 per CTA around its loop, 0.75 per tile,
+// whole rounds of two CTAs per SM. Clusters of 16 take 12 more and compete for the few places with 16 free
+// SMs: only where all of them run at once (8 units x 512 tiles 44 against 57 us with 8, but 32 units x 64
+// tiles 42 against 19 us).
+int few_cluster(long long units, int tiles, int head_dim, int sms) {
+    const double scale = head_dim == 64 ? 0.5 : 1.0;
+    double best = 0;
+    int pick = 1;
+    for (int c = 1; c <= pa::kFewMaxCluster && c <= tiles; c *= 2) {
+        const long long ctas = units * c;
+        if (c == 16 && ctas > sms) break;
+        const double loop = scale * ((tiles + c - 1) / c);
+        const double t = double((ctas + 2 * sms - 1) / (2 * sms)) * (loop * 0.75 + 7) + (c == 16 ? 12 : 0);
+        if (c == 1 || t < best) {
+            best = t;
+            pick = c;
+        }
+    }
+    return pick;
+}
+
 template <bool kBF16, int kD>
 int run_few(const pa_xattn_args* a, cudaStream_t s) {
     pa::XFewParams p;
@@ -58,19 +80,12 @@ int run_few(const pa_xattn_args* a, cudaStream_t s) {
     p.status = a->status;
     p.status_host = a->status_host;
     p.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;
-    // CTAs per (batch, kv head): as many as it takes to fill the GPU with two resident CTAs per SM,
-    // as long as each has a key tile.
     const long long units = static_cast<long long>(a->batch) * a->kv_heads;
     const int tiles = (a->seq_kv + pa::kFewKeys - 1) / pa::kFewKeys;
-    int c = 1;
-#ifdef PA_FEW_C
-    while (c < PA_FEW_C && 2 * c <= tiles) c *= 2;
-#else
-    while (c < pa::kFewMaxCluster && units * c < 2ll * sm_count() && 2 * c <= tiles) c *= 2;
-#endif
+    const int c = few_cluster(units, tiles, kD, sm_count());
     auto kern = pa::xattn_few_kernel<kBF16, kD>;
     const int smem = pa::few_smem_bytes<kD>();
-    const int rc = allow_smem(kern, smem, "xattn few rows");
+    const int rc = allow_smem(kern, smem, "xattn few rows", true);
     if (rc != PA_OK) return rc;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));

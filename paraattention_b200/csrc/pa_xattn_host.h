@@ -69,9 +69,9 @@ inline XattnMask xattn_mask_layout(const pa_xattn_args* a) {
     return m;
 }
 
-// Sets a kernel's shared-memory limit once per device.
+// Sets a kernel's shared-memory limit, and whether its clusters may have more than 8 CTAs, once per device.
 template <typename K>
-int allow_smem(K kern, int bytes, const char* what) {
+int allow_smem(K kern, int bytes, const char* what, bool wide_clusters = false) {
     static std::mutex mu;
     static const void* done[64][32] = {};
     int dev = 0;
@@ -84,6 +84,7 @@ int allow_smem(K kern, int bytes, const char* what) {
             if (d == nullptr) break;
         }
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return fail(PA_ECUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64)
         for (const void*& d : done[dev])

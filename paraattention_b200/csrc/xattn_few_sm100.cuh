@@ -6,7 +6,7 @@
 // hand-overs per key tile) costs microseconds before the first result; mma.sync m16n8k16 fits the
 // rows, keeps S, P and O in registers, and at 16 rows its rate is far above what HBM can feed.
 //
-// One cluster of 1, 2, 4 or 8 CTAs per (batch, kv head), the key tiles of 64 divided among its CTAs,
+// One cluster of 1 to 16 CTAs per (batch, kv head), the key tiles of 64 divided among its CTAs,
 // so that few heads still fill the GPU in ONE launch: the CTAs' partial results are joined through
 // distributed shared memory. Inside a CTA each of 4 warps owns 16 keys of every tile; 4 other warps
 // fill a 3-stage cp.async ring with K and V (the copies' addresses and the mask cost as many
@@ -28,8 +28,8 @@ namespace pa {
 constexpr int kFewRows = 16;
 constexpr int kFewKeys = 64;
 constexpr int kFewThreads = 128;  // that compute; as many more load
-constexpr int kFewStages = 3;
-constexpr int kFewMaxCluster = 8;
+constexpr int kFewStages = 3;  // (6 for CTAs that have an SM to themselves: no faster, the arithmetic is what they wait for)
+constexpr int kFewMaxCluster = 16;
 
 struct XFewParams {
     const uint16_t *q, *k, *v;
@@ -80,7 +80,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 template <bool kBF16, int kD>
-__global__ void __launch_bounds__(2 * kFewThreads)
+__global__ void __launch_bounds__(2 * kFewThreads, 2)
 xattn_few_kernel(const __grid_constant__ XFewParams p) {
     namespace cg = cooperative_groups;
     constexpr int kChunks = kD / 8;                 // 16-byte chunks of a row
