@@ -143,12 +143,12 @@ __device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u
     }
     return u.t1;
 }
-// The next segment that has steps, if any.
+// The unit of the next segment that has steps, if any.
 template <bool kKeys>
-__device__ __forceinline__ bool x_bwd_more(const XBwdParams& p, XCursor cursor) {
+__device__ __forceinline__ bool x_bwd_more(const XBwdParams& p, XCursor cursor, XBwdUnit& u) {
     XSeg g;
     while (cursor.next(p.sched, g)) {
-        const XBwdUnit u = x_bwd_unit<kKeys>(p, g);
+        u = x_bwd_unit<kKeys>(p, g);
         if (x_bwd_live<kKeys>(p, u, u.t0) < u.t1) return true;
     }
     return false;
@@ -460,6 +460,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         };
         bool ok = true;
         int j = 0, n_seg = 0;
+        float next_neg = 0.f, next_delta = 0.f;  // query pass: my row's statistics in the next segment with steps
+        float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
         while (ok && cursor.next(p.sched, seg)) {
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
@@ -470,11 +472,14 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 owe_release = true;
             }
             const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
-            float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
-            if (!kKeys) {
-                const float* r = row_stats(u);
-                neg.x = neg.y = __ldg(r);
-                dl.x = dl.y = __ldg(r + kTileN);
+            if (!kKeys && any) {
+                if (n_seg == 0) {
+                    const float* r = row_stats(u);
+                    next_neg = __ldg(r);
+                    next_delta = __ldg(r + kTileN);
+                }
+                neg = make_float2(next_neg, next_neg);
+                dl = make_float2(next_delta, next_delta);
             }
             const bool whole = p.words == nullptr && (!kKeys || (u.tile + 1) * kTileM <= p.skv);  // every owned key takes part
             while (st < u.t1) {
@@ -576,7 +581,11 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             if (any) {
                 // The last T2 is there, so X and Y in TMEM are free: the next segment's first products follow this
                 // one's last in the tensor core's queue and run during this one's epilogue.
-                if (!kKeys && x_bwd_more<kKeys>(p, cursor)) {
+                XBwdUnit next;
+                if (!kKeys && x_bwd_more<kKeys>(p, cursor, next)) {
+                    const float* r = row_stats(next);  // (its rows' statistics arrive meanwhile, too)
+                    next_neg = __ldg(r);
+                    next_delta = __ldg(r + kTileN);
                     ok = copy_xy();
                     if (!ok) break;
                     copied = true;
