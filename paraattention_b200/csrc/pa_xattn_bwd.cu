@@ -36,8 +36,11 @@ int pass(const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& z, const
     if (rc != PA_OK) return rc;
     kern<<<grid, pa::kXBwdThreads, pa::kXBwdSmemBytes, s>>>(x, y, z, w, g0, g1, p);
     rc = launched("xattn backward");
-    if (rc != PA_OK || !p.sched.split || grid == p.sched.team) return rc;
-    pa::xattn_bwd_join_kernel<kBF16, kD, kKeys><<<dim3(grid - p.sched.team, kD / 8, kKeys ? 2 : 1), 128, 0, s>>>(p, grid);
+    if (rc != PA_OK || !p.sched.split) return rc;
+    pa::XCutList cuts;
+    pa::x_list_cuts(p.sched, grid, &cuts);
+    if (cuts.n == 0) return PA_OK;
+    pa::xattn_bwd_join_kernel<kBF16, kD, kKeys><<<dim3(cuts.n, kD / 8, kKeys ? 2 : 1), 128, 0, s>>>(p, cuts);
     return launched("xattn backward join");
 }
 

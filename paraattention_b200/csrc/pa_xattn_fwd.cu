@@ -151,8 +151,11 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     if (rc != PA_OK) return rc;
     kern<<<f.grid, pa::kXFwdThreads, pa::kXFwdSmemBytes, s>>>(mq, mk, mv, mo, p);
     rc = launched("xattn forward");
-    if (rc != PA_OK || !f.sched.split || f.grid == f.sched.team) return rc;
-    pa::xattn_fwd_join_kernel<kBF16, kD><<<dim3(f.grid - f.sched.team, kD / 8), 256, 0, s>>>(p, f.grid);
+    if (rc != PA_OK || !f.sched.split) return rc;
+    pa::XCutList cuts;
+    pa::x_list_cuts(f.sched, f.grid, &cuts);
+    if (cuts.n == 0) return PA_OK;
+    pa::xattn_fwd_join_kernel<kBF16, kD><<<dim3(cuts.n, kD / 8), 256, 0, s>>>(p, cuts);
     return launched("xattn forward join");
 }
 

@@ -45,6 +45,7 @@ inline int xattn_sizes(const pa_xattn_args* a) {
 // `extra` steps' time and a thirty-second of the whole. `shared`: consecutive units that walk the same streamed tiles; they form teams
 // unless that leaves more than one SM in sixteen without work.
 inline pa::XSched xattn_schedule(long long units, long long steps, int shared, int sms, int extra, int* grid) {
+    sms = std::min(sms, pa::kXMaxCtas);
     pa::XSched s;
     s.units = static_cast<int>(units);
     s.steps = static_cast<int>(steps);

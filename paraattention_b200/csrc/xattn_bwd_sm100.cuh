@@ -663,9 +663,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 // cut unit, 8 columns and accumulator, one thread per row.
 template <bool kBF16, int kD, bool kKeys>
 __global__ void __launch_bounds__(128)
-xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, int grid) {
-    XCut cut;
-    if (!x_cut_unit(p.sched, blockIdx.x, grid, cut)) return;
+xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, const __grid_constant__ XCutList cuts) {
+    const XCut cut = cuts.cut[blockIdx.x];
     const int unit = cut.unit, cols0 = blockIdx.y * 8, which = blockIdx.z, r = threadIdx.x;
     float acc[8];
 #pragma unroll

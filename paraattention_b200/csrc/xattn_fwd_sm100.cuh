@@ -477,9 +477,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 //   out = sum_i 2^((m_i - m) sl) O_i / sum_i 2^((m_i - m) sl) l_i
 template <bool kBF16, int kD>
 __global__ void __launch_bounds__(256)
-xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, int grid) {
-    XCut cut;
-    if (!x_cut_unit(p.sched, blockIdx.x, grid, cut)) return;
+xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, const __grid_constant__ XCutList cuts) {
+    const XCut cut = cuts.cut[blockIdx.x];
     const int unit = cut.unit, cols0 = blockIdx.y * 8, r256 = threadIdx.x;
     const float sl = p.scale_log2;
     float m = -INFINITY;

@@ -80,22 +80,34 @@ struct XCursor {
     }
 };
 
-// The units that have to be joined are those that a range begins inside of; a joining launch has (teams - 1) *
-// team blocks, one for each such beginning, of which the first one inside a unit does the work.
-// x_cut_unit: the unit of block `index`, or -1; x_for_parts: calls f(slot) for its parts in range order.
-// (No range is empty: the grid has at most as many teams as there are steps.)
+// The units that have to be joined are those that a range begins inside of, listed by the host (the joining
+// kernels' blocks would spend longer on finding theirs than on the sums). No range is empty: the grid has
+// at most as many teams as there are steps.
+constexpr int kXMaxCtas = 160;
 struct XCut {
-    int unit, first, last;  // teams that have a part of it
+    int unit;
+    short first, last;  // teams that have a part of it
 };
-__device__ __forceinline__ bool x_cut_unit(const XSched& s, int index, int grid, XCut& cut) {
-    const int teams = grid / s.team, c = 1 + index / s.team;
-    const long long pos = x_range_begin(s, c, teams), row = pos / s.steps, a = row * s.steps;
-    if (pos == a || x_range_begin(s, c - 1, teams) > a) return false;
-    cut.unit = static_cast<int>(row) * s.team + index % s.team;
-    cut.first = c - 1;
-    cut.last = x_team_of(s, a + s.steps - 1, teams);
-    return true;
+struct XCutList {
+    int n;
+    XCut cut[kXMaxCtas];
+};
+inline void x_list_cuts(const XSched& s, int grid, XCutList* list) {
+    list->n = 0;
+    const int teams = grid / s.team;
+    for (int c = 1; c < teams; ++c) {
+        const long long pos = x_range_begin(s, c, teams), row = pos / s.steps, a = row * s.steps;
+        if (pos == a || x_range_begin(s, c - 1, teams) > a) continue;  // between units, or not the first cut of its unit
+        const int last = x_team_of(s, a + s.steps - 1, teams);
+        for (int m = 0; m < s.team; ++m) {
+            XCut& k = list->cut[list->n++];
+            k.unit = static_cast<int>(row) * s.team + m;
+            k.first = static_cast<short>(c - 1);
+            k.last = static_cast<short>(last);
+        }
+    }
 }
+// Calls f(slot) for the parts of a cut unit, in range order.
 template <typename F>
 __device__ __forceinline__ void x_for_parts(const XSched& s, const XCut& cut, F f) {
     const int member = cut.unit % s.team;
