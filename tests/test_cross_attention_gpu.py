@@ -375,6 +375,51 @@ def test_what_lies_behind_the_tensors_is_left_alone():
         assert bool(big_q[:, rows:].isnan().all()) and bool(big_k[:, Skv:].isnan().all())
 
 
+def test_a_reported_timeout_stops_later_calls_until_it_is_reset():
+    """The device's status word (set here by hand, as a wait that gave up would): tile kernels return at once and
+    leave their outputs alone; the host's word makes the next call raise; both are cleared by a reset."""
+    from paraattention_b200 import _lib as L
+    from paraattention_b200 import _status
+
+    q, k, v, do = make(1, 2, 2, 300, 200, 64, grad=True)
+    want = check_gradients(q, k, v, do)
+    recorded = ops.cross_attention(q, k, v)
+    mirror = _status.single_gpu_status(q.device)
+    try:
+        mirror.word.fill_(L.PA_DEV_TIMEOUT_PIPE)
+        out, lse = ops.cross_attention(q.detach(), k.detach(), v.detach(), return_lse=True)
+        torch.cuda.synchronize()
+        mirror.host.fill_(L.PA_DEV_TIMEOUT_PIPE)
+        with pytest.raises(L.PaError) as e:
+            ops.cross_attention(q.detach(), k.detach(), v.detach())
+        assert e.value.code == L.PA_ETIMEDOUT
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            torch.autograd.grad(recorded, (q, k, v), do)
+    finally:
+        mirror.reset()
+    again = check_gradients(q, k, v, do)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_first_call_inside_a_capture():
+    """Without a status word made yet, a captured call does without one."""
+    from paraattention_b200 import _status
+
+    q, k, v, _ = make(1, 2, 2, 200, 300, 64)
+    want = ops.cross_attention(q, k, v)
+    kept = dict(_status._single)
+    _status._single.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.cross_attention(q, k, v)
+        assert not _status._single
+    finally:
+        _status._single.update(kept)
+    graph.replay()
+    assert torch.equal(out, want)
+
+
 def test_refusals():
     q, k, v, _ = make(2, 4, 2, 5, 7, 64)
     with pytest.raises(NotImplementedError, match="bfloat16 and float16"):
