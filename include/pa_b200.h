@@ -240,8 +240,8 @@ int pa_qkv_prep(const pa_qkv_prep_args* args, void* stream);
  * LSE of -inf and no gradient; a key that no query sees has zero gradients.
  *
  * pa_xattn_fwd writes out and, if non-NULL, lse [batch, heads, seq_q] (fp32, natural log).
- * pa_xattn_bwd reads q, k, v, out, lse (of the forward call) and dout and writes dq, dk, dv whole;
- * with kv_batch = 1 dk and dv are the sums over the batch. Sums are fp32 in a fixed order: equal
+ * pa_xattn_bwd reads q, k, v, out, lse (of the forward call) and dout and writes dq, dk, dv whole
+ * (dq may be NULL, or dk and dv: not wanted, and not computed); with kv_batch = 1 dk and dv are the sums over the batch. Sums are fp32 in a fixed order: equal
  * calls on equal devices give equal bits.
  *
  * workspace: pa_xattn_workspace_bytes(args, backward) bytes (0 possible; depends on the current

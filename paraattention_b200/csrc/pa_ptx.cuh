@@ -141,9 +141,7 @@ __device__ __forceinline__ void tma_store_5d(const CUtensorMap* m, uint32_t src,
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 // The shared memory of every earlier store of this thread has been read / every store has completed.
-// (kLeft: but for the last kLeft of them)
-template <int kLeft = 0>
-__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory"); }
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

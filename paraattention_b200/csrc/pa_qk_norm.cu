@@ -64,7 +64,7 @@ int fill(const pa_qk_norm_args* a, bool backward, pa::QkNormParams* p) {
     const long long lines = static_cast<long long>(a->batch) * a->rows;
     const long long warps = static_cast<long long>(max_ctas()) * pa::kQkNormWarps;
     const int vec = 256 / a->head_dim;  // head vectors of one warp-wide access
-    const int most = (std::max(p->heads[0], p->heads[1]) + vec - 1) / vec;
+    const int most = std::min((std::max(p->heads[0], p->heads[1]) + vec - 1) / vec, 4096);
     double best = 0;
     for (int c = 1; c <= most; ++c) {
         const long long rounds = (lines * c + warps - 1) / warps;

@@ -180,27 +180,35 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
             at::AutoDispatchBelowADInplaceOrView below;
             at::NoGradGuard no_grad;
             c10::cuda::CUDAGuard guard(query.device());
-            Tensor dq = bshd(query), dk = bshd(key), dv = bshd(value);
+            // two passes, one for dq and one for dk and dv: each only if something is asked of it
+            const bool queries = ctx->needs_input_grad(0), keys = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+            Tensor dq, dk, dv;
+            if (queries) dq = bshd(query);
+            if (keys) dk = bshd(key), dv = bshd(value);
             if (query.numel() == 0 || key.numel() == 0) {
-                dq.zero_();
-                dk.zero_();
-                dv.zero_();
-            } else {
-                const Tensor q = ready(query), k = ready(key), v = ready(value), g = ready(dout);
-                pa_xattn_args a = cross_args(q, k, v, rows, out, lse, ctx->saved_data["scale"].toDouble());
+                for (Tensor* t : {&dq, &dk, &dv})
+                    if (t->defined()) t->zero_();
+            } else if (queries || keys) {
+                // (out may have been saved elsewhere meanwhile and come back with other strides)
+                const Tensor q = ready(query), k = ready(key), v = ready(value), g = ready(dout), o = ready(out);
+                pa_xattn_args a = cross_args(q, k, v, rows, o, lse, ctx->saved_data["scale"].toDouble());
                 a.dout = g.data_ptr();
-                a.dq = dq.data_ptr();
-                a.dk = dk.data_ptr();
-                a.dv = dv.data_ptr();
                 strides(g, a.do_stride);
-                strides(dq, a.dq_stride);
-                strides(dk, a.dk_stride);
-                strides(dv, a.dv_stride);
+                if (queries) {
+                    a.dq = dq.data_ptr();
+                    strides(dq, a.dq_stride);
+                }
+                if (keys) {
+                    a.dk = dk.data_ptr();
+                    a.dv = dv.data_ptr();
+                    strides(dk, a.dk_stride);
+                    strides(dv, a.dv_stride);
+                }
                 launch_cross(a, true, q, Status{ctx->saved_data["word"].toInt(), ctx->saved_data["host"].toInt()});
             }
             result[0] = dq;
             result[1] = dk;
-            result[2] = dv;
+            result[2] = dv;  // (what was not asked for is undefined, or dropped by the engine)
         }
         return once(std::move(result), "cross_attention");
     }

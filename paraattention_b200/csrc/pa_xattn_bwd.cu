@@ -51,9 +51,10 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     if (rc == PA_OK) rc = make_map(&mg, a->dout, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->do_stride[2], a->do_stride[1], a->do_stride[0], 0, "dout");
     if (rc == PA_OK) rc = make_map(&mk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k");
     if (rc == PA_OK) rc = make_map(&mv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v");
-    if (rc == PA_OK) rc = make_map(&mdq, a->dq, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->dq_stride[2], a->dq_stride[1], a->dq_stride[0], 0, "dq", 32, 32);
-    if (rc == PA_OK) rc = make_map(&mdk, a->dk, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dk_stride[2], a->dk_stride[1], a->dk_stride[0], 0, "dk", 32, 32);
-    if (rc == PA_OK) rc = make_map(&mdv, a->dv, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dv_stride[2], a->dv_stride[1], a->dv_stride[0], 0, "dv", 32, 32);
+    const bool queries = a->dq != nullptr, keys = a->dk != nullptr;
+    if (rc == PA_OK && queries) rc = make_map(&mdq, a->dq, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->dq_stride[2], a->dq_stride[1], a->dq_stride[0], 0, "dq", 32, 32);
+    if (rc == PA_OK && keys) rc = make_map(&mdk, a->dk, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dk_stride[2], a->dk_stride[1], a->dk_stride[0], 0, "dk", 32, 32);
+    if (rc == PA_OK && keys) rc = make_map(&mdv, a->dv, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dv_stride[2], a->dv_stride[1], a->dv_stride[0], 0, "dv", 32, 32);
     if (rc != PA_OK) return rc;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     pa::XBwdParams p;
@@ -102,13 +103,15 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     rc = launched("xattn row statistics");
     if (rc != PA_OK) return rc;
 
-    p.sched = f.k;
-    p.g[0] = static_cast<uint16_t*>(a->dk);
-    p.g[1] = static_cast<uint16_t*>(a->dv);
-    p.g_sb[0] = a->dk_stride[0]; p.g_sh[0] = a->dk_stride[1]; p.g_ss[0] = a->dk_stride[2];
-    p.g_sb[1] = a->dv_stride[0]; p.g_sh[1] = a->dv_stride[1]; p.g_ss[1] = a->dv_stride[2];
-    rc = pass<kBF16, kD, true>(mk, mv, mq, mg, mdk, mdv, p, f.grid_k, s);
-    if (rc != PA_OK) return rc;
+    if (keys) {
+        p.sched = f.k;
+        p.g[0] = static_cast<uint16_t*>(a->dk);
+        p.g[1] = static_cast<uint16_t*>(a->dv);
+        p.g_sb[0] = a->dk_stride[0]; p.g_sh[0] = a->dk_stride[1]; p.g_ss[0] = a->dk_stride[2];
+        p.g_sb[1] = a->dv_stride[0]; p.g_sh[1] = a->dv_stride[1]; p.g_ss[1] = a->dv_stride[2];
+        rc = pass<kBF16, kD, true>(mk, mv, mq, mg, mdk, mdv, p, f.grid_k, s);
+    }
+    if (rc != PA_OK || !queries) return rc;
     p.sched = f.q;
     p.g[0] = static_cast<uint16_t*>(a->dq);
     p.g[1] = nullptr;
@@ -129,10 +132,12 @@ int pa_xattn_bwd(const pa_xattn_args* a, void* stream) {
     if (rc == PA_OK) rc = xattn_tensor(a->v, a->v_stride, "v");
     if (rc == PA_OK) rc = xattn_tensor(a->out, a->o_stride, "out");
     if (rc == PA_OK) rc = xattn_tensor(a->dout, a->do_stride, "dout");
-    if (rc == PA_OK) rc = xattn_tensor(a->dq, a->dq_stride, "dq");
-    if (rc == PA_OK) rc = xattn_tensor(a->dk, a->dk_stride, "dk");
-    if (rc == PA_OK) rc = xattn_tensor(a->dv, a->dv_stride, "dv");
+    if (rc == PA_OK && a->dq != nullptr) rc = xattn_tensor(a->dq, a->dq_stride, "dq");
+    if (rc == PA_OK && a->dk != nullptr) rc = xattn_tensor(a->dk, a->dk_stride, "dk");
+    if (rc == PA_OK && a->dk != nullptr) rc = xattn_tensor(a->dv, a->dv_stride, "dv");
     if (rc != PA_OK) return rc;
+    if (a->dk == nullptr && (a->dv != nullptr || a->dq == nullptr))
+        return fail(PA_EINVAL, "xattn: the backward call computes dq, or dk and dv, or all three");
     if (a->lse == nullptr) return fail(PA_EINVAL, "xattn: the backward call needs the forward call's lse");
     const BwdPlan f = plan(a);
     if (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0 || a->workspace_bytes < f.bytes)

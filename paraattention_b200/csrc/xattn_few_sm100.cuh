@@ -222,9 +222,11 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
         for (int h = 0; h < 2; ++h) {
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            // (some key takes part, so mx is a number unless a logit is infinite itself)
-            alpha[h] = m[h] == -INFINITY ? 0.f : ex2_approx(m[h] - mx[h]);
+            // (keys that take part may have logits of -inf; 0 is then as good a reference as any)
+            const float ref = mx[h] == -INFINITY ? 0.f : mx[h];
+            alpha[h] = ex2_approx(m[h] - ref);
             m[h] = mx[h];
+            mx[h] = ref;
             l[h] *= alpha[h];
         }
         uint32_t pa_[4];
@@ -233,7 +235,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                e[i] = ex2_approx(s[nb][i] - m[i >> 1]);
+                e[i] = ex2_approx(s[nb][i] - mx[i >> 1]);
                 l[i >> 1] += e[i];
             }
             pa_[2 * nb] = kBF16 ? pack_bf16x2(e[0], e[1]) : pack_f16x2(e[0], e[1]);
@@ -285,7 +287,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float2 ml = wml[w * kFewRows + r];
-            wgt[w] = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mt);
+            wgt[w] = ml.y == 0.f ? 0.f : ex2_approx(ml.x - mt);
             lt += ml.y * wgt[w];
         }
         // (each element is read and written by the same thread)
@@ -316,7 +318,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
         for (int x = 0; x < 8; ++x) a[x] = 0.f;
         for (int k = 0; k < cn; ++k) {
             const float2 ml = cluster.map_shared_rank(cml, k)[r];
-            if (ml.x == -INFINITY) continue;
+            if (ml.y == 0.f) continue;  // (saw no key; a sum that is NaN stays one)
             const float wgt = ex2_approx(ml.x - mt);
             lt = fmaf(ml.y, wgt, lt);
             const float4* src = reinterpret_cast<const float4*>(cluster.map_shared_rank(wo, k) + r * kD + c0);
@@ -326,7 +328,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
             a[4] = fmaf(x1.x, wgt, a[4]); a[5] = fmaf(x1.y, wgt, a[5]);
             a[6] = fmaf(x1.z, wgt, a[6]); a[7] = fmaf(x1.w, wgt, a[7]);
         }
-        const float inv = lt > 0.f ? 1.f / lt : 0.f;
+        const float inv = lt != 0.f ? 1.f / lt : 0.f;
         const int g = r / p.sq, s = r - g * p.sq, head = hk * p.group + g;
         uint32_t w[4];
 #pragma unroll
@@ -335,7 +337,7 @@ xattn_few_kernel(const __grid_constant__ XFewParams p) {
         *reinterpret_cast<uint4*>(p.out + b * p.o_s[0] + head * p.o_s[1] + s * p.o_s[2] + c0) = make_uint4(w[0], w[1], w[2], w[3]);
         if (c0 == 0 && p.lse != nullptr)
             p.lse[(static_cast<long long>(b) * p.hkv * p.group + head) * p.sq + s] =
-                lt > 0.f ? 0.6931471805599453f * (mt + log2f(lt)) : -INFINITY;
+                lt != 0.f ? 0.6931471805599453f * (mt + log2f(lt)) : -INFINITY;
     }
     if (cn > 1) cluster.sync();  // (nobody leaves while its shared memory is still read)
 }

@@ -421,7 +421,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             const int tile = w.tile0 + t, g = tile / p.mt;
             const int row = (tile - g * p.mt) * kTileM + row_in_tile;
             const int head = w.hk * p.group + g;
-            const bool none = n <= 0 || !(l_sum > 0.0f);  // no key at all: zeros, LSE -inf
+            const bool none = n <= 0 || l_sum == 0.0f;  // no key at all: zeros, LSE -inf (a NaN sum stays one)
             const float inv = none ? 0.0f : 1.0f / l_sum;
             const int row_w = (tile - g * p.mt) * kTileM + quarter * 32;  // first of the warp's rows
 #pragma unroll 1
@@ -488,7 +488,7 @@ xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, const __grid_constan
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     x_for_parts(p.sched, cut, [&](int slot) {
         const float2 ml = __ldcg(p.part_ml + static_cast<long long>(slot) * 256 + r256);
-        if (ml.x == -INFINITY) return;  // (a share that saw no key)
+        if (ml.y == 0.f) return;  // (a share that saw no key)
         const float wgt = exp2f((ml.x - m) * sl);
         l += ml.y * wgt;
         const float4* src = reinterpret_cast<const float4*>(p.part_o) +
@@ -510,7 +510,7 @@ xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, const __grid_constan
     const int row = (tile - grp * p.mt) * kTileM + (r256 & 127);
     if (grp >= p.group || row >= p.sq) return;
     const int head = w.hk * p.group + grp;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
     uint16_t* orow = p.out + (w.b * p.o_sb + head * p.o_sh + row * p.o_ss) + cols0;
     uint32_t q[4];
 #pragma unroll
@@ -519,7 +519,7 @@ xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, const __grid_constan
     *reinterpret_cast<uint4*>(orow) = make_uint4(q[0], q[1], q[2], q[3]);
     if (blockIdx.y == 0 && p.lse != nullptr)
         p.lse[(static_cast<long long>(w.b) * p.hkv * p.group + head) * p.sq + row] =
-            l > 0.f ? m * p.scale + logf(l) : -INFINITY;
+            l != 0.f ? m * p.scale + logf(l) : -INFINITY;
 }
 
 }  // namespace pa

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from block_ops_reference import assert_within, cross_reference
 from paraattention_b200 import ops
@@ -331,6 +332,55 @@ def test_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("Sq,Skv", [(1, 100), (5, 333), (200, 300), (130, 4000)])
+def test_infinite_logits_and_nan_in_places_that_take_part(Sq, Skv):
+    """A key whose logits are -inf has weight zero, also where a whole run of keys is like that; NaN stays in the
+    rows that see it (the last size is divided over several CTAs)."""
+    q, k, v, _ = make(1, 2, 2, Sq, Skv, 64)
+    q[..., 0] = 1.0
+    k[:, :, :90, 0] = -math.inf
+    keep = torch.arange(Skv, device="cuda")[None] >= 90
+    kept = k.clone()
+    kept[:, :, :90, 0] = 0.0
+    out, lse = ops.cross_attention(q, k, v, return_lse=True)
+    want, bound = cross_reference(q, kept, v, keep, None)
+    assert_within(out, want["out"], bound["out"], "out")
+    assert_within(lse, want["lse"], bound["lse"], "lse")
+
+    q, k, v, do = make(1, 2, 2, Sq, Skv, 64, grad=True)
+    clean, clean_lse = ops.cross_attention(q, k, v, return_lse=True)
+    with torch.no_grad():
+        q[0, 0, Sq - 1, 3] = math.nan
+        k[0, 1, Skv - 1, 5] = math.nan
+    out, lse = ops.cross_attention(q, k, v, return_lse=True)
+    assert out[0, 0, Sq - 1].isnan().all() and lse[0, 0, Sq - 1].isnan() and out[0, 1].isnan().all() and lse[0, 1].isnan().all()
+    assert torch.equal(out[0, 0, :Sq - 1], clean[0, 0, :Sq - 1]) and torch.equal(lse[0, 0, :Sq - 1], clean_lse[0, 0, :Sq - 1])
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    assert dq[0, 0, Sq - 1].isnan().all() and dk[0, 0].isnan().all() and dv[0, 0].isnan().all() and dq[0, 1].isnan().all()
+    assert not dq[0, 0, :Sq - 1].isnan().any()
+
+
+@pytest.mark.parametrize("asked", [(0,), (1,), (2,), (0, 2), (1, 2)])
+@pytest.mark.parametrize("Sq", [1, 300])
+def test_gradients_alone_equal_those_of_the_whole_call(Sq, asked):
+    q, k, v, do = make(2, 4, 2, Sq, 200, 128, grad=True)
+    whole = check_gradients(q, k, v, do)[1:]
+    xs = [x if i in asked else x.detach() for i, x in enumerate((q, k, v))]
+    got = torch.autograd.grad(ops.cross_attention(*xs), [xs[i] for i in asked], do)
+    assert all(torch.equal(a, whole[i]) for a, i in zip(got, asked))
+
+
+def test_tensors_saved_elsewhere_between_forward_and_backward():
+    q, k, v, do = make(2, 4, 2, 300, 200, 64, grad=True)
+    mask = masks(2, 200)["holes"].cuda()
+    want = check_gradients(q, k, v, do, mask)[1:]
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        out = ops.cross_attention(q, k, v, mask)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (q, k, v), do), want))
+    out = torch.utils.checkpoint.checkpoint(lambda *a: ops.cross_attention(*a), q, k, v, mask, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (q, k, v), do), want))
 
 
 @pytest.mark.parametrize("Sq", [3, 200])
