@@ -103,20 +103,20 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     rc = launched("xattn row statistics");
     if (rc != PA_OK) return rc;
 
-    if (keys) {
-        p.sched = f.k;
-        p.g[0] = static_cast<uint16_t*>(a->dk);
-        p.g[1] = static_cast<uint16_t*>(a->dv);
-        p.g_sb[0] = a->dk_stride[0]; p.g_sh[0] = a->dk_stride[1]; p.g_ss[0] = a->dk_stride[2];
-        p.g_sb[1] = a->dv_stride[0]; p.g_sh[1] = a->dv_stride[1]; p.g_ss[1] = a->dv_stride[2];
-        rc = pass<kBF16, kD, true>(mk, mv, mq, mg, mdk, mdv, p, f.grid_k, s);
+    if (queries) {
+        p.sched = f.q;
+        p.g[0] = static_cast<uint16_t*>(a->dq);
+        p.g[1] = nullptr;
+        p.g_sb[0] = a->dq_stride[0]; p.g_sh[0] = a->dq_stride[1]; p.g_ss[0] = a->dq_stride[2];
+        rc = pass<kBF16, kD, false>(mq, mg, mk, mv, mdq, mdq, p, f.grid_q, s);
     }
-    if (rc != PA_OK || !queries) return rc;
-    p.sched = f.q;
-    p.g[0] = static_cast<uint16_t*>(a->dq);
-    p.g[1] = nullptr;
-    p.g_sb[0] = a->dq_stride[0]; p.g_sh[0] = a->dq_stride[1]; p.g_ss[0] = a->dq_stride[2];
-    return pass<kBF16, kD, false>(mq, mg, mk, mv, mdq, mdq, p, f.grid_q, s);
+    if (rc != PA_OK || !keys) return rc;
+    p.sched = f.k;
+    p.g[0] = static_cast<uint16_t*>(a->dk);
+    p.g[1] = static_cast<uint16_t*>(a->dv);
+    p.g_sb[0] = a->dk_stride[0]; p.g_sh[0] = a->dk_stride[1]; p.g_ss[0] = a->dk_stride[2];
+    p.g_sb[1] = a->dv_stride[0]; p.g_sh[1] = a->dv_stride[1]; p.g_ss[1] = a->dv_stride[2];
+    return pass<kBF16, kD, true>(mk, mv, mq, mg, mdk, mdv, p, f.grid_k, s);
 }
 
 }  // namespace
