@@ -69,6 +69,9 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     p.kt = f.kt;
     p.scale = a->scale;
     p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.by_group = pa::x_div(p.group);
+    p.by_mt = pa::x_div(f.mt);
+    p.by_b_steps = pa::x_div(p.group * f.mt);
     p.stats = reinterpret_cast<float*>(ws + f.off_stats);
     p.part = reinterpret_cast<float*>(ws + f.off_part);
     p.status = a->status;
@@ -105,6 +108,8 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
 
     if (queries) {
         p.sched = f.q;
+        p.by_tiles = pa::x_div(f.mt);
+        p.by_heads = pa::x_div(a->heads);
         p.g[0] = static_cast<uint16_t*>(a->dq);
         p.g[1] = nullptr;
         p.g_sb[0] = a->dq_stride[0]; p.g_sh[0] = a->dq_stride[1]; p.g_ss[0] = a->dq_stride[2];
@@ -112,6 +117,8 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     }
     if (rc != PA_OK || !keys) return rc;
     p.sched = f.k;
+    p.by_tiles = pa::x_div(f.kt);
+    p.by_heads = pa::x_div(a->kv_heads);
     p.g[0] = static_cast<uint16_t*>(a->dk);
     p.g[1] = static_cast<uint16_t*>(a->dv);
     p.g_sb[0] = a->dk_stride[0]; p.g_sh[0] = a->dk_stride[1]; p.g_ss[0] = a->dk_stride[2];

@@ -129,6 +129,9 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     p.o_sh = a->o_stride[1];
     p.o_ss = a->o_stride[2];
     p.sched = f.sched;
+    p.by_pairs = pa::x_div((p.group * f.mt + 1) / 2);
+    p.by_hkv = pa::x_div(p.hkv);
+    p.by_mt = pa::x_div(f.mt);
     p.status = a->status;
     p.status_host = a->status_host;
     p.wait_ns = a->wait_limit_ns ? a->wait_limit_ns : 2000000000ull;

@@ -60,6 +60,8 @@ struct XBwdParams {
     const unsigned long long* words;
     const int* extent;
     XSched sched;
+    XDiv by_tiles, by_heads;           // of the owned tensors
+    XDiv by_group, by_mt, by_b_steps;  // by_b_steps: the key pass's steps of a batch entry
     float* part;      // [slot][A1, A2][D / 4][128 rows][4]
     int* status;
     int* status_host;
@@ -99,12 +101,10 @@ struct XBwdStep {
 template <bool kKeys>
 __device__ __forceinline__ XBwdUnit x_bwd_unit(const XBwdParams& p, const XSeg& g) {
     XBwdUnit u;
-    int x = g.unit;
-    const int tiles = kKeys ? p.kt : p.mt, heads = kKeys ? p.hkv : p.hkv * p.group;
-    u.tile = x % tiles;
-    x /= tiles;
-    u.head = x % heads;
-    u.b = x / heads;
+    const int x = p.by_tiles(g.unit);
+    u.tile = g.unit - x * static_cast<int>(p.by_tiles.d);
+    u.b = p.by_heads(x);
+    u.head = x - u.b * static_cast<int>(p.by_heads.d);
     u.t0 = g.t0;
     u.t1 = g.t1;
     if (!kKeys && p.extent != nullptr) {  // key tiles behind the last key that takes part
@@ -120,13 +120,13 @@ __device__ __forceinline__ XBwdStep x_bwd_step(const XBwdParams& p, const XBwdUn
     XBwdStep s;
     if (!kKeys) {
         s.b = p.kv_batch == 1 ? 0 : u.b;
-        s.head = u.head / p.group;
+        s.head = p.by_group(u.head);
         s.tile = step;
         return s;
     }
-    const int m = step / p.mt;
+    const int m = p.by_mt(step);
     s.tile = step - m * p.mt;
-    const int bb = m / p.group;
+    const int bb = p.by_group(m);
     s.head = u.head * p.group + (m - bb * p.group);
     s.b = p.kv_batch == 1 ? bb : u.b;
     return s;
@@ -138,7 +138,7 @@ __device__ __forceinline__ int x_bwd_live(const XBwdParams& p, const XBwdUnit& u
     if (!kKeys || p.extent == nullptr) return step;
     const int per_b = p.group * p.mt;
     while (step < u.t1) {
-        const int b = p.kv_batch == 1 ? step / per_b : u.b;
+        const int b = p.kv_batch == 1 ? p.by_b_steps(step) : u.b;
         if (u.tile * kTileN < __ldg(p.extent + b)) return step;
         if (p.kv_batch != 1) return u.t1;
         step = (b + 1) * per_b;
@@ -526,7 +526,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                             const int c = i + 2 * y;
                             const float2 x = __ffma2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])), sl2, ng[y]);
                             float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
-                            if (!decltype(all)::value) {
+                            if (!decltype(all)::value && !(kKeys && plain)) {
                                 if (((live >> c) & 1u) == 0) e0 = 0.f;
                                 if (((live >> (c + 1)) & 1u) == 0) e1 = 0.f;
                             }
@@ -535,7 +535,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                         }
                     }
                 };
-                if (plain) weights(std::true_type());
+                if (!kKeys && plain) weights(std::true_type());
                 else weights(std::false_type());
                 if (kKeys) {
                     uint32_t pp[16];
@@ -568,7 +568,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                             const int c = i + 2 * y;
                             float2 s = __fmul2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])),
                                                   __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dt[y]));
-                            if (!decltype(all)::value) {  // (T2 of a masked key may be anything)
+                            if (!decltype(all)::value && !(kKeys && plain)) {  // (T2 of a masked key may be anything)
                                 if (((live >> c) & 1u) == 0) s.x = 0.f;
                                 if (((live >> (c + 1)) & 1u) == 0) s.y = 0.f;
                             }
@@ -576,7 +576,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                         }
                     }
                 };
-                if (plain) slopes(std::true_type());
+                if (!kKeys && plain) slopes(std::true_type());
                 else slopes(std::false_type());
                 tmem_st16(t2, ds);
                 tc_wait_st();

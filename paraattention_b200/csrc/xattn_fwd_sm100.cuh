@@ -44,6 +44,7 @@ struct XFwdParams {
     const unsigned long long* words;  // key mask, or NULL
     const int* extent;
     XSched sched;
+    XDiv by_pairs, by_hkv, by_mt;  // pairs: of row tiles of a (batch entry, kv head)
     float* part_o;    // [slot][D / 4][256 rows][4]
     float2* part_ml;  // [slot][256 rows] (reference, row sum)
     int* status;
@@ -73,13 +74,11 @@ struct XFwdUnit {
     int lo, hi;        // key tiles
 };
 __device__ __forceinline__ XFwdUnit x_fwd_unit(const XFwdParams& p, const XSeg& g) {
-    const int tiles = p.group * p.mt, pairs = (tiles + 1) >> 1;
     XFwdUnit u;
-    int x = g.unit;
-    u.tile0 = 2 * (x % pairs);
-    x /= pairs;
-    u.hk = x % p.hkv;
-    u.b = x / p.hkv;
+    const int x = p.by_pairs(g.unit);
+    u.tile0 = 2 * (g.unit - x * static_cast<int>(p.by_pairs.d));
+    u.b = p.by_hkv(x);
+    u.hk = x - u.b * p.hkv;
     u.lo = g.t0;
     u.hi = g.t1;
     if (p.extent != nullptr) {
@@ -167,7 +166,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     // (a second tile that does not exist is loaded from behind the last row: zeros)
-                    const int i = w.tile0 + t, g = i / p.mt;
+                    const int i = w.tile0 + t, g = p.by_mt(i);
                     const bool real = g < p.group;
                     const int row = real ? (i - g * p.mt) * kTileM : p.mt * kTileM;
 #pragma unroll
@@ -418,7 +417,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             *mine = l_sum;
             meet();
             l_sum += *other;
-            const int tile = w.tile0 + t, g = tile / p.mt;
+            const int tile = w.tile0 + t, g = p.by_mt(tile);
             const int row = (tile - g * p.mt) * kTileM + row_in_tile;
             const int head = w.hk * p.group + g;
             const bool none = n <= 0 || l_sum == 0.0f;  // no key at all: zeros, LSE -inf (a NaN sum stays one)
@@ -506,7 +505,7 @@ xattn_fwd_join_kernel(const __grid_constant__ XFwdParams p, const __grid_constan
     g.unit = unit;
     g.t0 = g.t1 = 0;
     const XFwdUnit w = x_fwd_unit(p, g);
-    const int tile = w.tile0 + (r256 >> 7), grp = tile / p.mt;
+    const int tile = w.tile0 + (r256 >> 7), grp = p.by_mt(tile);
     const int row = (tile - grp * p.mt) * kTileM + (r256 & 127);
     if (grp >= p.group || row >= p.sq) return;
     const int head = w.hk * p.group + grp;
