@@ -46,12 +46,13 @@ int pass(const CUtensorMap& x, const CUtensorMap& y, const CUtensorMap& z, const
 
 template <bool kBF16, int kD>
 int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
-    CUtensorMap mq, mk, mv, mg, mdq, mdk, mdv;  // (boxes of 128 x 64 for loads, 32 x 32 for stores)
+    CUtensorMap mq, mk, mv, mg, mo, mdq, mdk, mdv;  // (boxes of 128 x 64 for loads, 32 x 32 for stores)
     int rc = make_map(&mq, a->q, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->q_stride[2], a->q_stride[1], a->q_stride[0], 0, "q");
     if (rc == PA_OK) rc = make_map(&mg, a->dout, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->do_stride[2], a->do_stride[1], a->do_stride[0], 0, "dout");
     if (rc == PA_OK) rc = make_map(&mk, a->k, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->k_stride[2], a->k_stride[1], a->k_stride[0], 0, "k");
     if (rc == PA_OK) rc = make_map(&mv, a->v, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->v_stride[2], a->v_stride[1], a->v_stride[0], 0, "v");
     const bool queries = a->dq != nullptr, keys = a->dk != nullptr;
+    if (rc == PA_OK && queries) rc = make_map(&mo, a->out, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->o_stride[2], a->o_stride[1], a->o_stride[0], 0, "out");
     if (rc == PA_OK && queries) rc = make_map(&mdq, a->dq, a->dtype, kD, a->seq_q, a->heads, a->batch, 1, a->dq_stride[2], a->dq_stride[1], a->dq_stride[0], 0, "dq", 32, 32);
     if (rc == PA_OK && keys) rc = make_map(&mdk, a->dk, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dk_stride[2], a->dk_stride[1], a->dk_stride[0], 0, "dk", 32, 32);
     if (rc == PA_OK && keys) rc = make_map(&mdv, a->dv, a->dtype, kD, a->seq_kv, a->kv_heads, a->kv_batch, 1, a->dv_stride[2], a->dv_stride[1], a->dv_stride[0], 0, "dv", 32, 32);
@@ -86,36 +87,39 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
         rc = launched("xattn mask");
         if (rc != PA_OK) return rc;
     }
-    pa::XStatParams st;
-    memset(&st, 0, sizeof(st));
-    st.o = static_cast<const uint16_t*>(a->out);
-    st.g = static_cast<const uint16_t*>(a->dout);
-    for (int i = 0; i < 3; ++i) {
-        st.o_s[i] = a->o_stride[i];
-        st.g_s[i] = a->do_stride[i];
-    }
-    st.lse = a->lse;
-    st.stats = const_cast<float*>(p.stats);
-    st.batch = a->batch;
-    st.heads = a->heads;
-    st.sq = a->seq_q;
-    st.padded = f.mt * 128;
-    const long long vectors = static_cast<long long>(a->batch) * a->heads * st.padded, per_cta = pa::kXStatThreads / (kD / 8) * 4;
-    const int stat_grid = static_cast<int>(std::min<long long>((vectors + per_cta - 1) / per_cta, 8ll * sm_count()));
-    pa::xattn_stat_kernel<kBF16, kD><<<stat_grid, pa::kXStatThreads, 0, s>>>(st);
-    rc = launched("xattn row statistics");
-    if (rc != PA_OK) return rc;
-
     if (queries) {
-        p.sched = f.q;
-        p.by_tiles = pa::x_div(f.mt);
-        p.by_heads = pa::x_div(a->heads);
-        p.g[0] = static_cast<uint16_t*>(a->dq);
-        p.g[1] = nullptr;
-        p.g_sb[0] = a->dq_stride[0]; p.g_sh[0] = a->dq_stride[1]; p.g_ss[0] = a->dq_stride[2];
-        rc = pass<kBF16, kD, false>(mq, mg, mk, mv, mdq, mdq, p, f.grid_q, s);
+        pa::XBwdParams pq = p;
+        pq.sched = f.q;
+        pq.by_tiles = pa::x_div(f.mt);
+        pq.by_heads = pa::x_div(a->heads);
+        pq.o = static_cast<const uint16_t*>(a->out);
+        for (int i = 0; i < 3; ++i) pq.o_s[i] = a->o_stride[i];
+        pq.lse = a->lse;
+        pq.g[0] = static_cast<uint16_t*>(a->dq);
+        pq.g_sb[0] = a->dq_stride[0]; pq.g_sh[0] = a->dq_stride[1]; pq.g_ss[0] = a->dq_stride[2];
+        rc = pass<kBF16, kD, false>(mq, mg, mk, mv, mdq, mo, pq, f.grid_q, s);
+        if (rc != PA_OK || !keys) return rc;
+    } else {
+        pa::XStatParams st;
+        memset(&st, 0, sizeof(st));
+        st.o = static_cast<const uint16_t*>(a->out);
+        st.g = static_cast<const uint16_t*>(a->dout);
+        for (int i = 0; i < 3; ++i) {
+            st.o_s[i] = a->o_stride[i];
+            st.g_s[i] = a->do_stride[i];
+        }
+        st.lse = a->lse;
+        st.stats = p.stats;
+        st.batch = a->batch;
+        st.heads = a->heads;
+        st.sq = a->seq_q;
+        st.padded = f.mt * 128;
+        const long long vectors = static_cast<long long>(a->batch) * a->heads * st.padded, per_cta = pa::kXStatThreads / (kD / 8) * 4;
+        const int stat_grid = static_cast<int>(std::min<long long>((vectors + per_cta - 1) / per_cta, 8ll * sm_count()));
+        pa::xattn_stat_kernel<kBF16, kD><<<stat_grid, pa::kXStatThreads, 0, s>>>(st);
+        rc = launched("xattn row statistics");
+        if (rc != PA_OK) return rc;
     }
-    if (rc != PA_OK || !keys) return rc;
     p.sched = f.k;
     p.by_tiles = pa::x_div(f.kt);
     p.by_heads = pa::x_div(a->kv_heads);

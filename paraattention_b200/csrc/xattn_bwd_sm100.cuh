@@ -55,8 +55,13 @@ struct XBwdParams {
     uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv (written with TMA, but for joined or empty tiles)
     long long g_sb[2], g_sh[2], g_ss[2];
     // [B][Hq][mt][-lse * log2 e, -delta][128 rows]; rows behind the last query, and rows without
-    // any key, have (-inf, 0), which makes their P zero
-    const float* stats;
+    // any key, have (-inf, 0), which makes their P zero. Read by the key pass; written by the query pass if
+    // there is one, which has do on the SM anyway (97 us more for it, against 122 us for a kernel of its own, at
+    // 32760 x 512 x 40 heads; 8 against 14 us at 2 x 2049 x 333 x 32 heads), else by xattn_stat_kernel.
+    float* stats;
+    const uint16_t* o;  // query pass: out
+    long long o_s[3];
+    const float* lse;   // query pass: [B][Hq][Sq]
     const unsigned long long* words;
     const int* extent;
     XSched sched;
@@ -71,6 +76,7 @@ struct XBwdParams {
 struct XBwdCtl {
     uint64_t xy_full, xy_empty;
     uint64_t xt_full;               // query pass: X and Y are in TMEM (one arrival per warp)
+    uint64_t stat_full;             // query pass: lse and do * out of the owned rows are in `stat` (one arrival per warp)
     uint64_t z_full[kXZStages], z_empty[kXZStages], z_clean[kXZStages];
     uint64_t w_full[kXWStages], w_empty[kXWStages];
     uint64_t t1_full, t2_full;
@@ -82,7 +88,7 @@ struct XBwdCtl {
     uint32_t tmem_base;
     int abort;
 };
-// Operands, the key pass's ring of row statistics, control block. (The dynamic shared memory is declared with the
+// Operands, row statistics, control block. (The dynamic shared memory is declared with the
 // alignment of the swizzle; there is no room for slack.)
 constexpr int kXBwdStatBytes = kXWStages * kTileN * 8;
 constexpr int kXBwdSmemBytes = (2 + kXZStages + kXWStages) * kTileBytes + kXBwdStatBytes + 512;
@@ -156,6 +162,18 @@ __device__ __forceinline__ bool x_bwd_more(const XBwdParams& p, XCursor cursor, 
     return false;
 }
 
+// Sum of the products of two chunks of 8 elements.
+template <bool kBF16>
+__device__ __forceinline__ float dot8(const uint32_t* x, const uint32_t* y) {
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        dot = fmaf(lo16<kBF16>(x[i]), lo16<kBF16>(y[i]), dot);
+        dot = fmaf(hi16<kBF16>(x[i]), hi16<kBF16>(y[i]), dot);
+    }
+    return dot;
+}
+
 template <bool kBF16, int kD, bool kKeys>
 __global__ void __launch_bounds__(kXBwdThreads, 1)
 xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y,
@@ -169,7 +187,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sZ + kXZStages * kTileBytes;
     uint8_t* smem_z = smem + 2 * kTileBytes;
-    float* stat = reinterpret_cast<float*>(smem + (2 + kXZStages + kXWStages) * kTileBytes);  // [W stage][2][128], key pass
+    // key pass: [W stage][2][128], a step's row statistics; query pass: [2][128], lse and do * out of the owned rows
+    float* stat = reinterpret_cast<float*>(smem + (2 + kXZStages + kXWStages) * kTileBytes);
     XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + (2 + kXZStages + kXWStages) * kTileBytes + kXBwdStatBytes);
     volatile int* s_abort = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -189,6 +208,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         mbar_init(smem_u32(&ctl->xy_full), 1);
         mbar_init(smem_u32(&ctl->xy_empty), kXBwdSoftWarps);
         mbar_init(smem_u32(&ctl->xt_full), kXBwdSoftWarps);
+        mbar_init(smem_u32(&ctl->stat_full), kXBwdSoftWarps);
         for (int s = 0; s < kXZStages; ++s) {
             mbar_init(smem_u32(&ctl->z_full[s]), 1);
             mbar_init(smem_u32(&ctl->z_empty[s]), 1);
@@ -250,6 +270,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 for (int h = 0; h < kAtoms; ++h) {
                     tma_load_5d(sX + h * kHalfBytes, &tm_x, bx, h * 64, u.tile * kTileM, u.head, u.b, 0);
                     tma_load_5d(sY + h * kHalfBytes, &tm_y, bx, h * 64, u.tile * kTileM, u.head, u.b, 0);
+                    if (!kKeys) tma_prefetch_5d(&tm_g1, h * 64, u.tile * kTileM, u.head, u.b, 0);  // (out)
                 }
                 for (; st < u.t1; st = x_bwd_live<kKeys>(p, u, st + 1), ++j) {
                     const XBwdStep s = x_bwd_step<kKeys>(p, u, st);
@@ -425,9 +446,23 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             if (lane == 0) mbar_arrive(smem_u32(bar));
         };
         // Query pass: brings a segment's X and Y from shared memory to TMEM once its predecessor's products
-        // are done. D / 8 16-byte chunks per row, four of them per warp.
+        // are done: D / 8 16-byte chunks per row, four of them per warp. Then adds up do * out of the rows, each warp
+        // for 8 of them, with whole rows per load (from registers, where a thread has a quarter of a row of do, the
+        // loads of out take 32 lines each and the pass 35 us longer) and in the order of xattn_stat_kernel, so
+        // that dk and dv do not depend on who adds up.
         int n_copied = 0;
-        auto copy_xy = [&]() -> bool {
+        auto copy_xy = [&](const XBwdUnit& w) -> bool {
+            constexpr int kLanes = kD / 8, kRows = 32 / kLanes, kTurns = 8 / kRows;
+            const int chunk = lane % kLanes, dot_row = warp * 8 + lane / kLanes;  // in the tile; kRows on with every turn
+            uint4 o[kTurns];
+            const uint16_t* from = p.o + (w.b * p.o_s[0] + w.head * p.o_s[1]) + chunk * 8;
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int row = w.tile * kTileM + dot_row + i * kRows;
+                o[i] = row < p.sq ? __ldg(reinterpret_cast<const uint4*>(from + row * p.o_s[2])) : make_uint4(0, 0, 0, 0);
+            }
+            const int lse_row = w.tile * kTileM + warp * 8 + (lane & 7);  // (behind the last query: as without any key)
+            const float lse = lse_row < p.sq ? __ldg(p.lse + (static_cast<long long>(w.b) * p.hkv * p.group + w.head) * p.sq + lse_row) : -INFINITY;
             if (!wait(&ctl->xy_full, n_copied & 1)) return false;
             if (piece * 4 < kD / 8) {
 #pragma unroll
@@ -445,11 +480,20 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             }
             tc_fence_before();
             arrive(&ctl->xt_full);
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int r = dot_row + i * kRows;
+                const uint4 y = *reinterpret_cast<const uint4*>(smem + kTileBytes + (chunk >> 3) * kHalfBytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+                const uint32_t xs[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, ys[4] = {y.x, y.y, y.z, y.w};
+                float dot = dot8<kBF16>(xs, ys);
+#pragma unroll
+                for (int k = 1; k < kLanes; k <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
+                if (chunk == 0) stat[kTileM + r] = dot;
+            }
+            if (lane < 8) stat[warp * 8 + lane] = lse;
+            arrive(&ctl->stat_full);
             ++n_copied;
             return true;
-        };
-        auto row_stats = [&](const XBwdUnit& u) -> const float* {
-            return p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt + u.tile) * (2 * kTileN) + row_in_tile;
         };
         // Tells the producer that the owned tiles' memory may be loaded again (the stores staged there have been read).
         bool owe_release = false;
@@ -462,26 +506,30 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         };
         bool ok = true;
         int j = 0, n_seg = 0;
-        float next_neg = 0.f, next_delta = 0.f;  // query pass: my row's statistics in the next segment with steps
         float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
         while (ok && cursor.next(p.sched, seg)) {
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
             const bool any = st < u.t1;
             if (!kKeys && any && n_seg == 0) {
-                ok = copy_xy();
+                ok = copy_xy(u);
                 if (!ok) break;
                 owe_release = true;
             }
             const int row = u.tile * kTileM + row_in_tile;  // my query (query pass) or key (key pass)
             if (!kKeys && any) {
-                if (n_seg == 0) {
-                    const float* r = row_stats(u);
-                    next_neg = __ldg(r);
-                    next_delta = __ldg(r + kTileN);
+                ok = wait(&ctl->stat_full, n_seg & 1);
+                if (!ok) break;
+                const float lse = stat[row_in_tile], dot = stat[kTileM + row_in_tile];
+                const bool none = lse == -INFINITY;
+                const float n1 = none ? -INFINITY : lse * -1.4426950408889634f, d1 = none ? 0.f : -dot;
+                neg = make_float2(n1, n1);
+                dl = make_float2(d1, d1);
+                if (piece == 0 && u.t0 == 0) {  // for the key pass (a unit has one segment with its first step)
+                    float* dst = p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt + u.tile) * (2 * kTileN) + row_in_tile;
+                    dst[0] = n1;
+                    dst[kTileN] = d1;
                 }
-                neg = make_float2(next_neg, next_neg);
-                dl = make_float2(next_delta, next_delta);
             }
             const bool whole = p.words == nullptr && (!kKeys || (u.tile + 1) * kTileM <= p.skv);  // every owned key takes part
             while (st < u.t1) {
@@ -595,10 +643,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 // one's last in the tensor core's queue and run during this one's epilogue.
                 XBwdUnit next;
                 if (!kKeys && x_bwd_more<kKeys>(p, cursor, next)) {
-                    const float* r = row_stats(next);  // (its rows' statistics arrive meanwhile, too)
-                    next_neg = __ldg(r);
-                    next_delta = __ldg(r + kTileN);
-                    ok = copy_xy();
+                    ok = copy_xy(next);
                     if (!ok) break;
                     copied = true;
                 }
@@ -610,9 +655,9 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 ++n_seg;
             }
             // Each warp writes blocks of 32 rows x 32 columns: the query pass's one of dq, the key pass's two of dk and
-            // dv; staged where the owned tiles were, which are no longer needed.
+            // dv; staged where the owned tiles (query pass: X alone) were, which are no longer needed.
             constexpr int kBlocks = (kKeys ? 2 : 1) * kD / 32;  // of 32 columns
-            static_assert(kXBwdSoftWarps * ((kBlocks + 3) / 4) * kXStageBytes <= 2 * kTileBytes, "the staging fits");
+            static_assert(kXBwdSoftWarps * ((kBlocks + 3) / 4) * kXStageBytes <= (kKeys ? 2 : 1) * kTileBytes, "the staging fits");
             const int row_w = u.tile * kTileM + quarter * 32, rows = kKeys ? p.skv : p.sq;
 #pragma unroll
             for (int blk = piece; blk < kBlocks; blk += 4) {
@@ -635,7 +680,7 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                     for (int x = 0; x < 32; ++x) o[x] = 0u;
                 }
                 if (seg.slot < 0) {
-                    uint8_t* stage = smem + (warp * 2 + blk / 4) * kXStageBytes;
+                    uint8_t* stage = smem + (warp * (kKeys ? 2 : 1) + blk / 4) * kXStageBytes;
                     x_stage32<kBF16>(stage, lane, o, which ? 1.0f : p.scale);
                     fence_proxy_async_shared();
                     __syncwarp();
@@ -709,7 +754,8 @@ xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, const __grid_constan
 }
 
 // stats[b][h][tile][0 / 1][128] = -lse * log2 e and -sum_d do * out of the query rows; (-inf, 0) for rows without
-// any key and behind the last one. HBM-bound: one pass over do and out, 16 bytes per lane.
+// any key and behind the last one; for calls without a query pass. HBM-bound: one pass over do and out, 16 bytes
+// per lane.
 struct XStatParams {
     const uint16_t *o, *g;  // out, do
     long long o_s[3], g_s[3];
@@ -751,14 +797,9 @@ xattn_stat_kernel(const __grid_constant__ XStatParams p) {
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
             const uint32_t xs[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, ys[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-            float dot = 0.f;
+            float dot = dot8<kBF16>(xs, ys);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                dot = fmaf(lo16<kBF16>(xs[i]), lo16<kBF16>(ys[i]), dot);
-                dot = fmaf(hi16<kBF16>(xs[i]), hi16<kBF16>(ys[i]), dot);
-            }
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            for (int o = 1; o < kLanes; o <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
             if (at == 0 && to[u] != ~0u) {
                 const bool none = l[u] == -INFINITY;
                 float* dst = p.stats + static_cast<long long>(to[u] / kTileN) * (2 * kTileN) + to[u] % kTileN;

@@ -32,8 +32,8 @@ struct XSched {
 
 // Division of 0 <= x < 2^31 by a constant of the launch: with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), which
 // is below 2^32, m d - 2^(31 + l) < d <= 2^l, so x m / 2^(31 + l) exceeds x / d by less than 1 / d. (The roles
-// find their way from unit to unit with it; with the / operator that took 1200 of the query pass's 12500 cycles a
-// unit.)
+// find their way from unit to unit with it: with the / operator the backward kernel's query pass took 478
+// instead of 464 us at 32760 x 512 x 40 heads.)
 struct XDiv {
     unsigned d, mul;
     int shift;
