@@ -80,6 +80,18 @@ def test_cross_attention_validates_before_any_launch(lib):
     assert lib.pa_xattn_bwd(C.byref(a), None) == L.PA_EINVAL
 
 
+def test_cross_attention_backward_of_one_side(lib):
+    """dq alone and dk with dv get as far as the missing workspace; nothing at all, or half a pair, do not."""
+    buf = (C.c_uint8 * 256)()
+    addr = (C.addressof(buf) + 15) // 16 * 16
+    for gone, what in ((("dq",), b"workspace"), (("dk", "dv"), b"workspace"), (("dq", "dk", "dv"), b"computes"),
+                       (("dk",), b"computes"), (("dv",), b"dv"), (("dq", "dv"), b"dv")):
+        a = _xattn(addr)
+        for field in gone:
+            setattr(a, field, None)
+        assert lib.pa_xattn_bwd(C.byref(a), None) == L.PA_EINVAL and what in lib.pa_last_error(), gone
+
+
 def test_cross_attention_workspace_sizes(lib):
     a = _xattn(0)
     assert lib.pa_xattn_workspace_bytes(C.byref(a), 0) == 0  # few tiles of keys: nothing to divide
