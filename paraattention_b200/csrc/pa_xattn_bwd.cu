@@ -9,7 +9,8 @@ namespace {
 struct BwdPlan {
     pa::XSched q, k;  // query pass, key pass
     int grid_q = 0, grid_k = 0, mt = 0, kt = 0;
-    int64_t off_stats = 0, off_part = 0, bytes = 0;
+    int bound_parts = 0, bound_keys = 0;  // f16: parts of a key head's values and their keys (a multiple of 64)
+    int64_t off_stats = 0, off_do_max = 0, off_v_max = 0, off_part = 0, bytes = 0;
 };
 
 BwdPlan plan(const pa_xattn_args* a) {
@@ -22,6 +23,14 @@ BwdPlan plan(const pa_xattn_args* a) {
                          static_cast<long long>(a->batch / a->kv_batch) * (a->heads / a->kv_heads) * f.mt, f.kt, sms, 4, &f.grid_k);
     f.off_stats = xattn_mask_layout(a).bytes;
     f.off_part = f.off_stats + int64_t(a->batch) * a->heads * f.mt * 128 * 8;
+    if (a->dtype == PA_F16) {
+        const int64_t shared = int64_t(a->kv_batch) * a->kv_heads;
+        f.bound_keys = ((a->seq_kv + pa::kXBoundParts - 1) / pa::kXBoundParts + 63) / 64 * 64;
+        f.bound_parts = (a->seq_kv + f.bound_keys - 1) / f.bound_keys;
+        f.off_do_max = f.off_part;
+        f.off_v_max = f.off_do_max + up256(shared * 4);
+        f.off_part = f.off_v_max + up256(shared * pa::kXBoundParts * 4);
+    }
     // (the passes run one after the other and use the same partial results' space)
     const int64_t slots = std::max(f.q.split ? 2 * f.grid_q : 0, f.k.split ? 2 * f.grid_k : 0);
     f.bytes = f.off_part + slots * 2 * 128 * a->head_dim * 4;
@@ -87,6 +96,26 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
         rc = launched("xattn mask");
         if (rc != PA_OK) return rc;
     }
+    if constexpr (!kBF16) {
+        pa::XBoundParams bp;
+        memset(&bp, 0, sizeof(bp));
+        bp.v = static_cast<const uint16_t*>(a->v);
+        for (int i = 0; i < 3; ++i) bp.v_s[i] = a->v_stride[i];
+        bp.words = p.words;
+        bp.batch = a->batch;
+        bp.kv_batch = a->kv_batch;
+        bp.hkv = a->kv_heads;
+        bp.skv = a->seq_kv;
+        bp.keys = f.bound_keys;
+        bp.v_max = reinterpret_cast<unsigned*>(ws + f.off_v_max);
+        bp.do_max = reinterpret_cast<unsigned*>(ws + f.off_do_max);
+        p.v_max = bp.v_max;
+        p.do_max = bp.do_max;
+        p.v_parts = f.bound_parts;
+        pa::xattn_bound_kernel<kD><<<dim3(a->kv_batch * a->kv_heads, f.bound_parts), pa::kXBoundThreads, 0, s>>>(bp);
+        rc = launched("xattn bounds");
+        if (rc != PA_OK) return rc;
+    }
     if (queries) {
         pa::XBwdParams pq = p;
         pq.sched = f.q;
@@ -114,6 +143,10 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
         st.heads = a->heads;
         st.sq = a->seq_q;
         st.padded = f.mt * 128;
+        st.do_max = p.do_max;
+        st.kv_batch = a->kv_batch;
+        st.hkv = a->kv_heads;
+        st.by_group = p.by_group;
         const long long vectors = static_cast<long long>(a->batch) * a->heads * st.padded, per_cta = pa::kXStatThreads / (kD / 8) * 4;
         const int stat_grid = static_cast<int>(std::min<long long>((vectors + per_cta - 1) / per_cta, 8ll * sm_count()));
         pa::xattn_stat_kernel<kBF16, kD><<<stat_grid, pa::kXStatThreads, 0, s>>>(st);

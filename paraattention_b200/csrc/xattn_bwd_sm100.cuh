@@ -32,8 +32,17 @@
 // (xattn_sm100.cuh divides the work).
 //
 // What is rounded: P and dS to the tensors' 16-bit type, as operands of a 16-bit product (their
-// relative error, half an ulp, averages out over the sum; in f16, values below 2^-14 have steps of 2^-24, so
-// a weight of 1 / 32760 is off by 2^-10 of itself at most, less than any bf16 weight); everything else is fp32.
+// relative error, half an ulp, averages out over the sum); everything else is fp32. bf16 has fp32's range. f16
+// has not: below 2^-14 its steps are 2^-24, whatever the value, and dS, about |do| / Skv times ten, is there for
+// ordinary gradients (8192 keys, do of 1e-3: dq off by 7.6e-3 of itself); above 65504 it is infinite. So in f16 both
+// are powers of two larger or smaller than they are, and the epilogue takes that back, exactly, from the fp32 sums:
+//   P by 2^14 (P <= 1);
+//   dS by 2^e with |dS| 2^e < 2^15. |dS| <= P (|dP| + |delta|) <= 2 sum|do| max|v|, since out is an average of values;
+//     sum over a row of do, max over the values of the key head that take part. The query pass has an e of its own for
+//     each row; the key pass, which adds up over rows, has the one of the key head's largest row.
+// max|v| comes from a launch in front (xattn_bound_kernel), sum|do| from where the row statistics are made. What is
+// not finite takes no part in the bounds: it makes its own results so, and no other's. The half steps of dS are then at
+// most 2^-39 of that bound. (Masked values take no part either: they may hold anything.)
 #pragma once
 #include <type_traits>
 
@@ -48,6 +57,9 @@ constexpr int kXBwdThreads = 640;
 // Z is needed from T1 to A1, W from T2 to A2 or less: three stages of Z and two of W leave every load
 // the time of five products.
 constexpr int kXZStages = 3, kXWStages = 2;
+// f16: the exponent of P, and how many parts of a key head's values the launch in front of the passes bounds by themselves.
+constexpr int kXShiftP = 14;
+constexpr int kXBoundParts = 32;
 
 struct XBwdParams {
     int batch, kv_batch, hkv, group, sq, skv;
@@ -55,7 +67,7 @@ struct XBwdParams {
     float scale, scale_log2;
     uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv (written with TMA, but for joined or empty tiles)
     long long g_sb[2], g_sh[2], g_ss[2];
-    // [B][Hq][mt][-lse * log2 e, -delta][128 rows]; rows behind the last query, and rows without
+    // [B][Hq][mt][-lse * log2 e (f16: + kXShiftP), -delta][128 rows]; rows behind the last query, and rows without
     // any key, have (-inf, 0), which makes their P zero. Read by the key pass; written by the query pass if
     // there is one, which has do on the SM anyway (97 us more for it, against 122 us for a kernel of its own, at
     // 32760 x 512 x 40 heads; 8 against 14 us at 2 x 2049 x 333 x 32 heads), else by xattn_stat_kernel.
@@ -63,6 +75,11 @@ struct XBwdParams {
     const uint16_t* o;  // query pass: out
     long long o_s[3];
     const float* lse;   // query pass: [B][Hq][Sq]
+    // f16: per [kv batch][kv head], the largest |v| of each part of its keys and the largest sum|do| of a row of its
+    // queries (float bits; written by the query pass or xattn_stat_kernel, read by the key pass)
+    const unsigned* v_max;  // [][kXBoundParts], the first v_parts written
+    unsigned* do_max;
+    int v_parts;
     const unsigned long long* words;
     const int* extent;
     XSched sched;
@@ -175,6 +192,26 @@ __device__ __forceinline__ float dot8(const uint32_t* x, const uint32_t* y) {
     return dot;
 }
 
+// Sum of the magnitudes of a chunk of 8 elements.
+template <bool kBF16>
+__device__ __forceinline__ float abs8(const uint32_t* x) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += fabsf(lo16<kBF16>(x[i])) + fabsf(hi16<kBF16>(x[i]));
+    return sum;
+}
+// f16: the exponent e with 2 bound 2^e in [2^14, 2^15) (bound: a product of sums and values of f16 numbers, so 2^-48
+// to 2^40 if it is finite and not zero), and 2^-e.
+__device__ __forceinline__ int x_slope_exp(float bound) {
+    return bound > 0.f && bound < INFINITY ? 13 - (static_cast<int>(__float_as_uint(bound) >> 23) - 127) : 0;
+}
+__device__ __forceinline__ float x_pow2(int e) { return __uint_as_float(static_cast<unsigned>(127 + e) << 23); }
+// The largest |v| of a (kv batch, kv head). A whole warp calls.
+__device__ __forceinline__ float x_v_max(const XBwdParams& p, int unit, int lane) {
+    const unsigned m = lane < p.v_parts ? __ldg(p.v_max + static_cast<long long>(unit) * kXBoundParts + lane) : 0u;
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+}
+
 template <bool kBF16, int kD, bool kKeys>
 __global__ void __launch_bounds__(kXBwdThreads, 1)
 xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y,
@@ -188,7 +225,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sX = smem_u32(smem), sY = sX + kTileBytes, sZ = sX + 2 * kTileBytes, sW = sZ + kXZStages * kTileBytes;
     uint8_t* smem_z = smem + 2 * kTileBytes;
-    // key pass: [W stage][2][128], a step's row statistics; query pass: [2][128], lse and do * out of the owned rows
+    // key pass: [W stage][2][128], a step's row statistics; query pass: [3][128], lse and do * out of the owned rows and,
+    // in f16, the exponent of their dS
     float* stat = reinterpret_cast<float*>(smem + (2 + kXZStages + kXWStages) * kTileBytes);
     XBwdCtl* ctl = reinterpret_cast<XBwdCtl*>(smem + (2 + kXZStages + kXWStages) * kTileBytes + kXBwdStatBytes);
     volatile int* s_abort = &ctl->abort;
@@ -481,6 +519,10 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             }
             tc_fence_before();
             arrive(&ctl->xt_full);
+            const int shared_by = (p.kv_batch == 1 ? 0 : w.b) * p.hkv + p.by_group(w.head);  // (f16)
+            float v_max = 0.f;
+            unsigned largest = 0u;
+            if constexpr (!kBF16) v_max = x_v_max(p, shared_by, lane);
 #pragma unroll
             for (int i = 0; i < kTurns; ++i) {
                 const int r = dot_row + i * kRows;
@@ -490,6 +532,19 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 #pragma unroll
                 for (int k = 1; k < kLanes; k <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, k);
                 if (chunk == 0) stat[kTileM + r] = dot;
+                if constexpr (!kBF16) {
+                    float sum = abs8<kBF16>(ys);
+#pragma unroll
+                    for (int k = 1; k < kLanes; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+                    if (chunk == 0) stat[2 * kTileM + r] = static_cast<float>(x_slope_exp(sum * v_max));
+                    // (rows without any key: as in xattn_stat_kernel)
+                    const float its_lse = __shfl_sync(0xffffffffu, lse, lane / kLanes + i * kRows);
+                    if (sum < INFINITY && its_lse != -INFINITY) largest = max(largest, __float_as_uint(sum));
+                }
+            }
+            if constexpr (!kBF16) {
+                largest = __reduce_max_sync(0xffffffffu, largest);
+                if (lane == 0) atomicMax(p.do_max + shared_by, largest);
             }
             if (lane < 8) stat[warp * 8 + lane] = lse;
             arrive(&ctl->stat_full);
@@ -508,6 +563,9 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         bool ok = true;
         int j = 0, n_seg = 0;
         float2 neg = make_float2(0.f, 0.f), dl = make_float2(0.f, 0.f);
+        // f16: query pass, 2^-e of my row, which A1 is to be multiplied by; key pass, 2^(e - kXShiftP), which makes dS of
+        // P (dP - delta) with P as it is handed over
+        float shift = 1.f;
         while (ok && cursor.next(p.sched, seg)) {
             const XBwdUnit u = x_bwd_unit<kKeys>(p, seg);
             int st = x_bwd_live<kKeys>(p, u, u.t0);
@@ -523,14 +581,26 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 if (!ok) break;
                 const float lse = stat[row_in_tile], dot = stat[kTileM + row_in_tile];
                 const bool none = lse == -INFINITY;
-                const float n1 = none ? -INFINITY : lse * -1.4426950408889634f, d1 = none ? 0.f : -dot;
+                float n1 = none ? -INFINITY : __fmul_rn(lse, -1.4426950408889634f);
+                const float d1 = none ? 0.f : -dot;
                 neg = make_float2(n1, n1);
                 dl = make_float2(d1, d1);
+                if constexpr (!kBF16) {  // (here P is in dS alone)
+                    const float e = stat[2 * kTileM + row_in_tile];
+                    neg = make_float2(n1 + e, n1 + e);
+                    shift = x_pow2(-static_cast<int>(e));
+                    n1 = __fadd_rn(n1, kXShiftP);
+                }
                 if (piece == 0 && u.t0 == 0) {  // for the key pass (a unit has one segment with its first step)
                     float* dst = p.stats + ((static_cast<long long>(u.b) * p.hkv * p.group + u.head) * p.mt + u.tile) * (2 * kTileN) + row_in_tile;
                     dst[0] = n1;
                     dst[kTileN] = d1;
                 }
+            }
+            if constexpr (!kBF16 && kKeys) {
+                const int unit = u.b * p.hkv + u.head;
+                const int e = x_slope_exp(__uint_as_float(__ldcg(p.do_max + unit)) * x_v_max(p, unit, lane));
+                shift = x_pow2(e - kXShiftP);
             }
             const bool whole = p.words == nullptr && (!kKeys || (u.tile + 1) * kTileM <= p.skv);  // every owned key takes part
             while (st < u.t1) {
@@ -615,8 +685,9 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             const int c = i + 2 * y;
-                            float2 s = __fmul2_rn(make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1])),
-                                                  __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dt[y]));
+                            float2 w = make_float2(__uint_as_float(a[c]), __uint_as_float(a[c + 1]));
+                            if constexpr (!kBF16 && kKeys) w = __fmul2_rn(w, make_float2(shift, shift));
+                            float2 s = __fmul2_rn(w, __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dt[y]));
                             if (!decltype(all)::value && !(kKeys && plain)) {  // (T2 of a masked key may be anything)
                                 if (((live >> c) & 1u) == 0) s.x = 0.f;
                                 if (((live >> (c + 1)) & 1u) == 0) s.y = 0.f;
@@ -660,6 +731,9 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             constexpr int kBlocks = (kKeys ? 2 : 1) * kD / 32;  // of 32 columns
             static_assert(kXBwdSoftWarps * ((kBlocks + 3) / 4) * kXStageBytes <= (kKeys ? 2 : 1) * kTileBytes, "the staging fits");
             const int row_w = u.tile * kTileM + quarter * 32, rows = kKeys ? p.skv : p.sq;
+            // (2^-e from 2^(e - kXShiftP): a difference of exponents)
+            const float undo = kBF16 ? 1.0f : kKeys ? __uint_as_float((static_cast<unsigned>(254 - kXShiftP) << 23) - __float_as_uint(shift)) : shift;
+            const float undo_p = kBF16 ? 1.0f : x_pow2(-kXShiftP);
 #pragma unroll
             for (int blk = piece; blk < kBlocks; blk += 4) {
                 const int which = blk / (kD / 32), col = blk % (kD / 32) * 32;
@@ -682,12 +756,16 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 }
                 if (seg.slot < 0) {
                     uint8_t* stage = smem + (warp * (kKeys ? 2 : 1) + blk / 4) * kXStageBytes;
-                    x_stage32<kBF16>(stage, lane, o, which ? 1.0f : p.scale);
+                    x_stage32<kBF16>(stage, lane, o, which ? undo_p : p.scale * undo);
                     fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0 && row_w < rows)
                         tma_store_5d(which ? &tm_g1 : &tm_g0, smem_u32(stage), col, row_w, u.head, u.b, 0);
                 } else {
+                    if constexpr (!kBF16) {  // (the joining kernel adds up what the values are)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * (which ? undo_p : undo));
+                    }
                     float4* part = reinterpret_cast<float4*>(p.part) +
                                    ((static_cast<long long>(seg.slot) * 2 + which) * (kD / 4) + col / 4) * kTileM + row_in_tile;
 #pragma unroll
@@ -754,7 +832,55 @@ xattn_bwd_join_kernel(const __grid_constant__ XBwdParams p, const __grid_constan
     *reinterpret_cast<uint4*>(grow) = make_uint4(q[0], q[1], q[2], q[3]);
 }
 
-// stats[b][h][tile][0 / 1][128] = -lse * log2 e and -sum_d do * out of the query rows; (-inf, 0) for rows without
+// f16: v_max[kv batch][kv head][part] = the largest finite |v| of the keys of the part that take part in any batch entry
+// that shares them, and a cleared do_max. One block per (kv batch, kv head) and part, 16 bytes per lane, HBM-bound:
+// v is read once more. 2.2 us for 2 x 77 keys x 16 heads of 64, 4.9 us for 512 keys x 40 heads of 128; where v is the largest
+// tensor it shows (256 queries x 32760 keys x 24 heads: the backward call takes 516 instead of 474 us).
+struct XBoundParams {
+    const uint16_t* v;
+    long long v_s[3];
+    const unsigned long long* words;
+    int batch, kv_batch, hkv, skv;
+    int keys;  // of a part
+    unsigned *v_max, *do_max;
+};
+constexpr int kXBoundThreads = 256;
+template <int kD>
+__global__ void __launch_bounds__(kXBoundThreads)
+xattn_bound_kernel(const __grid_constant__ XBoundParams p) {
+    constexpr int kLanes = kD / 8;
+    __shared__ unsigned of_warp[kXBoundThreads / 32];
+    const int b = blockIdx.x / p.hkv, h = blockIdx.x - b * p.hkv, n_words = (p.skv + 63) >> 6;
+    const int first = blockIdx.y * p.keys, end = min(first + p.keys, p.skv);
+    const int b0 = p.kv_batch == 1 ? 0 : b, b1 = p.kv_batch == 1 ? p.batch : b + 1;
+    const uint16_t* from = p.v + b * p.v_s[0] + h * p.v_s[1] + threadIdx.x % kLanes * 8;
+    float m = 0.f;
+#pragma unroll 4
+    for (int key = first + threadIdx.x / kLanes; key < end; key += kXBoundThreads / kLanes) {
+        bool live = p.words == nullptr;
+        for (int bb = b0; bb < b1 && !live; ++bb)
+            live = ((__ldg(p.words + static_cast<long long>(bb) * n_words + (key >> 6)) >> (key & 63)) & 1ull) != 0;
+        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(from + key * p.v_s[2])) : make_uint4(0, 0, 0, 0);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lo = fabsf(lo16<false>(xs[i])), hi = fabsf(hi16<false>(xs[i]));
+            m = fmaxf(m, fmaxf(lo < INFINITY ? lo : 0.f, hi < INFINITY ? hi : 0.f));
+        }
+    }
+    const unsigned w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = w;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned all = of_warp[0];
+#pragma unroll
+        for (int i = 1; i < kXBoundThreads / 32; ++i) all = max(all, of_warp[i]);
+        p.v_max[static_cast<long long>(blockIdx.x) * kXBoundParts + blockIdx.y] = all;
+        if (blockIdx.y == 0) p.do_max[blockIdx.x] = 0u;
+    }
+}
+
+// stats[b][h][tile][0 / 1][128] = -lse * log2 e (in f16, + the exponent of P) and -sum_d do * out of the query rows; (-inf, 0) for rows without
 // any key and behind the last one; for calls without a query pass. HBM-bound: one pass over do and out, 16 bytes
 // per lane.
 struct XStatParams {
@@ -762,9 +888,15 @@ struct XStatParams {
     long long o_s[3], g_s[3];
     const float* lse;  // [B][Hq][Sq]
     float* stats;      // [B][Hq][padded / 128][2][128]
+    unsigned* do_max;  // f16: XBwdParams::do_max
     int batch, heads, sq, padded;
+    int kv_batch, hkv;
+    XDiv by_group;
 };
 constexpr int kXStatThreads = 256;
+// f16: each CTA finds the largest rows of its key heads in shared memory first (a look at the global word for every
+// row made the kernel's 128 us 301 us at 32760 x 512 x 40 heads; so it is 149 us), if there are no more of them than this.
+constexpr int kXStatUnits = 1024;
 template <bool kBF16, int kD>
 __global__ void __launch_bounds__(kXStatThreads)
 xattn_stat_kernel(const __grid_constant__ XStatParams p) {
@@ -773,12 +905,20 @@ xattn_stat_kernel(const __grid_constant__ XStatParams p) {
     constexpr int kAtOnce = 4;  // vectors per lane in flight
     constexpr unsigned kGroups = kXStatThreads / kLanes;
     const unsigned n = static_cast<unsigned>(p.batch) * p.heads * p.padded;  // (the host has checked the range)
+    __shared__ unsigned most[kBF16 ? 1 : kXStatUnits];
+    const int units = p.kv_batch * p.hkv;
+    const bool here = units <= kXStatUnits;
+    if constexpr (!kBF16) {
+        for (int i = threadIdx.x; i < units && here; i += kXStatThreads) most[i] = 0u;
+        __syncthreads();
+    }
     // (heads innermost: neighbouring lanes read neighbouring heads of [B, S, H, D] memory. The trip count
     // is the same for all lanes of a warp - the shuffles need them all.)
     for (unsigned base = blockIdx.x * (kGroups * kAtOnce); base < n; base += gridDim.x * (kGroups * kAtOnce)) {
         uint4 x[kAtOnce], y[kAtOnce];
         float l[kAtOnce];
         unsigned to[kAtOnce];
+        int unit[kAtOnce];
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
             const unsigned idx = base + u * kGroups + threadIdx.x / kLanes;
@@ -788,6 +928,7 @@ xattn_stat_kernel(const __grid_constant__ XStatParams p) {
             const int s = static_cast<int>(t) - b * p.padded;
             x[u] = y[u] = make_uint4(0, 0, 0, 0);
             l[u] = -INFINITY;  // (behind the last query, as without any key)
+            unit[u] = kBF16 ? 0 : (p.kv_batch == 1 ? 0 : b) * p.hkv + p.by_group(h);
             to[u] = idx < n ? (static_cast<unsigned>(b) * p.heads + h) * p.padded + s : ~0u;
             if (idx < n && s < p.sq) {
                 x[u] = __ldg(reinterpret_cast<const uint4*>(p.o + (b * p.o_s[0] + h * p.o_s[1] + s * p.o_s[2]) + at));
@@ -801,13 +942,32 @@ xattn_stat_kernel(const __grid_constant__ XStatParams p) {
             float dot = dot8<kBF16>(xs, ys);
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            float sum = 0.f;
+            if constexpr (!kBF16) {
+                sum = abs8<kBF16>(ys);
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            }
             if (at == 0 && to[u] != ~0u) {
                 const bool none = l[u] == -INFINITY;
                 float* dst = p.stats + static_cast<long long>(to[u] / kTileN) * (2 * kTileN) + to[u] % kTileN;
-                dst[0] = none ? -INFINITY : l[u] * -1.4426950408889634f;
+                // (two roundings, as in the query pass)
+                const float n1 = __fmul_rn(l[u], -1.4426950408889634f);
+                dst[0] = none ? -INFINITY : kBF16 ? n1 : __fadd_rn(n1, kXShiftP);
                 dst[kTileN] = none ? 0.f : -dot;
+                if constexpr (!kBF16) {
+                    if (!none && sum < INFINITY) {
+                        if (here) atomicMax(most + unit[u], __float_as_uint(sum));
+                        else if (__float_as_uint(sum) > __ldcg(p.do_max + unit[u])) atomicMax(p.do_max + unit[u], __float_as_uint(sum));
+                    }
+                }
             }
         }
+    }
+    if constexpr (!kBF16) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < units && here; i += kXStatThreads)
+            if (most[i] != 0u) atomicMax(p.do_max + i, most[i]);
     }
 }
 
