@@ -5,7 +5,7 @@ rotation (``qk_norm_rotary``). Both are re-exported by :mod:`paraattention_b200.
 Like the other ops of this package they are CUDA-only, launch on the current stream, never
 synchronise, and raise instead of falling back. Both carry gradients: outside ``torch.no_grad()``,
 with an input that requires a gradient, the call is recorded and its backward pass is a kernel of
-libpa_b200 too (first derivatives only). The arguments are checked here; the rest of a call -
+libpa_b200 too (first derivatives in reverse mode only; a tensor with a forward-mode tangent is refused). The arguments are checked here; the rest of a call -
 output and scratch memory from PyTorch's caching allocator (so concurrent streams and captured
 graphs never share scratch), the C ABI's argument structures, the autograd node - is the extension
 _pa_torch.so (csrc/pa_torch.cpp).

@@ -38,6 +38,16 @@ void check(int rc, bool backward) {
     if (rc != PA_OK) raise(rc, backward);
 }
 
+// These operators have no forward-mode rule. A tensor with a tangent need not require a gradient, and a result computed
+// below the autograd keys carries none, which PyTorch takes for zero: refused instead. (Not where forward mode is off, as in the
+// forward of a function that has a rule of its own.)
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
+                                    ": forward-mode derivatives are not built (an input has a tangent)");
+}
+
 // x itself if the kernels can address it in place (unit stride on head_dim, 16-byte aligned base and strides,
 // no broadcast dimensions), else a contiguous copy.
 Tensor ready(const Tensor& x) {
@@ -174,6 +184,7 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
         variable_list result(7);
         const Tensor dout = grads[0];
         if (!dout.defined()) return result;
+        refuse_tangents("the backward pass of cross_attention", {&dout});
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &query = saved[0], &key = saved[1], &value = saved[2], &rows = saved[3], &out = saved[4], &lse = saved[5];
         {
@@ -217,6 +228,7 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
 std::tuple<Tensor, std::optional<Tensor>> cross_attention(const Tensor& query, const Tensor& key, const Tensor& value,
                                                           const std::optional<Tensor>& rows_, double scale, bool need_lse,
                                                           int64_t word, int64_t host) {
+    refuse_tangents("cross_attention", {&query, &key, &value});
     if (at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad())) {
         auto r = CrossAttention::apply(query, key, value, rows_, scale, word, host);
         return {r[0], need_lse ? std::optional<Tensor>(r[1]) : std::nullopt};
@@ -308,6 +320,7 @@ struct QkNorm : public torch::autograd::Function<QkNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list result(9);
+        for (const Tensor& g : grads) refuse_tangents("the backward pass of qk_norm_rotary", {&g});
         const variable_list saved = ctx->get_saved_variables();
         const NormPlan plan{ctx->saved_data["row_offset"].toInt(), ctx->saved_data["interleaved"].toBool(),
                             ctx->saved_data["eps"].toDouble()};
@@ -372,18 +385,21 @@ std::tuple<Tensor, std::optional<Tensor>> qk_norm_rotary(const Tensor& q, const 
                                                          const std::optional<Tensor>& wq_, const std::optional<Tensor>& wk_,
                                                          const std::optional<Tensor>& cos_, const std::optional<Tensor>& sin_,
                                                          int64_t row_offset, bool interleaved, double eps) {
+    const Tensor k = k_.value_or(Tensor()), wq = wq_.value_or(Tensor()), wk = wk_.value_or(Tensor());
+    const Tensor cos = cos_.value_or(Tensor()), sin = sin_.value_or(Tensor());
+    refuse_tangents("qk_norm_rotary", {&q, &k, &wq, &wk, &cos, &sin});
     auto asks = [](const std::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
     variable_list ys;
     if (at::GradMode::is_enabled() && (q.requires_grad() || asks(k_) || asks(wq_) || asks(wk_))) {
         ys = QkNorm::apply(q, k_, wq_, wk_, cos_, sin_, row_offset, interleaved, eps);
     } else {
         at::AutoDispatchBelowADInplaceOrView below;
-        variable_list xs{q}, ws{wq_.value_or(Tensor())};
-        if (k_.has_value()) {
-            xs.push_back(*k_);
-            ws.push_back(wk_.value_or(Tensor()));
+        variable_list xs{q}, ws{wq};
+        if (k.defined()) {
+            xs.push_back(k);
+            ws.push_back(wk);
         }
-        ys = norm_forward(xs, ws, cos_.value_or(Tensor()), sin_.value_or(Tensor()), NormPlan{row_offset, interleaved, eps});
+        ys = norm_forward(xs, ws, cos, sin, NormPlan{row_offset, interleaved, eps});
     }
     return {ys[0], ys.size() > 1 ? std::optional<Tensor>(ys[1]) : std::nullopt};
 }
