@@ -12,7 +12,7 @@ NCCL path would raise or abort on a stuck collective. ``reset()`` clears both wo
 """
 from __future__ import annotations
 
-from typing import Dict, Optional
+from typing import Dict, List
 
 import torch
 
@@ -45,21 +45,37 @@ class StatusMirror:
         self.check()
 
     def reset(self) -> None:
+        """Clear both words. Waits for the device: launches in flight that found the old code report it first."""
         self.word.zero_()
+        if self.word.device.type == "cuda":
+            torch.cuda.synchronize(self.word.device)
         self.host.zero_()
 
 
 _single: Dict[int, StatusMirror] = {}
+_in_graphs: List[StatusMirror] = []  # made by first calls inside a capture; graphs hold their addresses
 
 
 def single_gpu_status(device: torch.device) -> StatusMirror:
     """The status word the single-GPU attention ops of this process share on ``device``."""
     m = _single.get(device.index)
-    if m is None:
-        m = StatusMirror(torch.zeros(1, dtype=torch.int32, device=device))
-        _single[device.index] = m
+    if m is not None:
+        return m
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            # This word is filled by the graph, in front of the launches that read it: it is the graph's alone.
+            m = StatusMirror(torch.zeros(1, dtype=torch.int32, device=device))
+            _in_graphs.append(m)
+            return m
+    # Launches on any stream read the word without waiting for this one, so it is filled before its address is
+    # known: on a stream of its own, which may be waited for while this one is busy.
+    stream = torch.cuda.Stream(device)
+    with torch.cuda.stream(stream):
+        word = torch.zeros(1, dtype=torch.int32, device=device)
+    stream.synchronize()
+    m = _single[device.index] = StatusMirror(word)
     return m
 
 
 def all_mirrors():
-    return list(_single.values())
+    return [*_single.values(), *_in_graphs]

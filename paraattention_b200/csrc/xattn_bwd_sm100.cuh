@@ -237,8 +237,8 @@ xattn_bwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         if ((sX & 1023u) != 0) {  // (never seen; the swizzled tiles would not be where the descriptors say)
             st = PA_DEV_TIMEOUT_PIPE;
             if (p.status != nullptr) atomicCAS(p.status, 0, st);
-            x_report(p.status_host, st);
         }
+        x_report(p.status_host, st);  // (a launch that does nothing because of an earlier one's wait says so, too)
         ctl->abort = st;
     }
     __syncthreads();
