@@ -23,9 +23,11 @@ class StatusMirror:
     def __init__(self, word: torch.Tensor):
         assert word.dtype == torch.int32 and word.numel() == 1
         self.word = word
-        host = torch.zeros(1, dtype=torch.int32)
-        # (pinning needs a CUDA runtime; a CPU word - the unit tests - gets a plain host copy)
-        self.host = host.pin_memory() if word.device.type == "cuda" else host
+        # (an ordinary tensor, also if the first call is made in inference mode: later ones write to it)
+        with torch.inference_mode(False):
+            host = torch.zeros(1, dtype=torch.int32)
+            # (pinning needs a CUDA runtime; a CPU word - the unit tests - gets a plain host copy)
+            self.host = host.pin_memory() if word.device.type == "cuda" else host
 
     def check(self) -> None:
         """Raise if an earlier launch reported a timed-out wait. Reads host memory only."""
@@ -61,7 +63,7 @@ def single_gpu_status(device: torch.device) -> StatusMirror:
     m = _single.get(device.index)
     if m is not None:
         return m
-    with torch.cuda.device(device):
+    with torch.cuda.device(device), torch.inference_mode(False):
         if torch.cuda.is_current_stream_capturing():
             # This word is filled by the graph, in front of the launches that read it: it is the graph's alone.
             m = StatusMirror(torch.zeros(1, dtype=torch.int32, device=device))
@@ -70,7 +72,7 @@ def single_gpu_status(device: torch.device) -> StatusMirror:
     # Launches on any stream read the word without waiting for this one, so it is filled before its address is
     # known: on a stream of its own, which may be waited for while this one is busy.
     stream = torch.cuda.Stream(device)
-    with torch.cuda.stream(stream):
+    with torch.cuda.stream(stream), torch.inference_mode(False):
         word = torch.zeros(1, dtype=torch.int32, device=device)
     stream.synchronize()
     m = _single[device.index] = StatusMirror(word)

@@ -88,3 +88,24 @@ def test_a_first_call_inside_a_capture_keeps_its_word_to_itself():
         torch.cuda.synchronize()
         _status._single.clear()
         _status._single.update(kept)
+
+
+def test_a_first_call_in_inference_mode():
+    """The status words it makes serve calls and resets outside of inference mode, too."""
+    dev = torch.device("cuda", torch.cuda.current_device())
+    kept = dict(_status._single)
+    q, k, v = make()
+    want = ops.cross_attention(q, k, v)
+    try:
+        _status._single.clear()
+        with torch.inference_mode():
+            assert torch.equal(ops.cross_attention(q, k, v), want)
+        ops.attention_forward(q, q, q)  # (queues a copy to the host's word)
+        assert torch.equal(ops.cross_attention(q, k, v), want)
+        torch.cuda.synchronize()
+        pa.reset_device_status()
+        assert torch.equal(ops.cross_attention(q, k, v), want) and dev.index in _status._single
+    finally:
+        torch.cuda.synchronize()
+        _status._single.clear()
+        _status._single.update(kept)
