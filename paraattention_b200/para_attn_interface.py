@@ -455,7 +455,10 @@ def cross_attn_func(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=
 
 class CrossAttnMode(_AttnModeBase):
     """Routes ``F.scaled_dot_product_attention`` calls whose keys are of another length than the queries
-    to ``cross_attn_func``; every other call passes. Under context parallelism, where each rank has its own
+    to ``cross_attn_func``; every other call passes on, to PyTorch or the mode around this one, and so do calls
+    in a form that ``cross_attn_func`` does not compute: masks that are not boolean key-padding masks, dropout,
+    ``is_causal``, other types than bf16 and f16, other head sizes than 64 and 128, tensors that are not
+    [B, H, S, D], forward-mode tangents. (Wrong arguments and CPU tensors raise.) Under context parallelism, where each rank has its own
     query rows and the whole prompt, such calls need no exchange: enter this mode outside a
     ``UnifiedAttnMode(mesh, skip_small_kv=True)``, which hands them on.
 
@@ -479,4 +482,9 @@ class CrossAttnMode(_AttnModeBase):
         return super().__torch_function__(func, types, args, kwargs)
 
     def _call_attn_func(self, *args, **kwargs):
-        return cross_attn_func(*args, **kwargs)
+        if all(t.ndim == 4 for t in _get_args(args, kwargs, "query", "key", "value")):
+            try:
+                return cross_attn_func(*args, **kwargs)
+            except NotImplementedError:
+                pass
+        return base_handle_torch_function(F.scaled_dot_product_attention, (), args, kwargs)
