@@ -148,8 +148,10 @@ std::tuple<Tensor, Tensor> cross_forward(const Tensor& query, const Tensor& key,
     return {out, lse};
 }
 
-// First derivatives only: differentiating the result once more raises.
-variable_list once(variable_list grads, const char* what) {
+// First derivatives only: differentiating the result once more raises. The node that raises hangs on everything the
+// gradients are functions of (`sources`), not on the gradients alone: where only the way to one input is walked, a node off that
+// way is not run, and PyTorch takes the derivative for zero.
+variable_list once(variable_list grads, const variable_list& sources, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
     std::vector<size_t> at_;
     variable_list defined;
@@ -159,6 +161,8 @@ variable_list once(variable_list grads, const char* what) {
             defined.push_back(grads[i].requires_grad() ? grads[i] : grads[i].detach().requires_grad_(true));
         }
     if (defined.empty()) return grads;
+    for (const Tensor& s : sources)
+        if (s.defined() && s.requires_grad()) defined.push_back(s);
     auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " can be differentiated once only",
                                                                   static_cast<int64_t>(defined.size()));
     variable_list marked = (*error)(std::move(defined));
@@ -221,7 +225,7 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
             result[1] = dk;
             result[2] = dv;  // (what was not asked for is undefined, or dropped by the engine)
         }
-        return once(std::move(result), "cross_attention");
+        return once(std::move(result), {dout, query, key, value}, "cross_attention");
     }
 };
 
@@ -377,7 +381,9 @@ struct QkNorm : public torch::autograd::Function<QkNorm> {
                 }
             }
         }
-        return once(std::move(result), "qk_norm_rotary");
+        variable_list sources(saved.begin(), saved.begin() + 4);
+        sources.insert(sources.end(), grads.begin(), grads.end());
+        return once(std::move(result), sources, "qk_norm_rotary");
     }
 };
 
