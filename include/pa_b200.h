@@ -299,7 +299,7 @@ typedef struct pa_qk_norm_args {
     const void* dy[2];       /* backward */
     void* y[2];              /* forward: outputs; backward: dx */
     const void* weight[2];
-    void* dweight[2];        /* backward, each may be NULL */
+    void* dweight[2];        /* backward, each may be NULL (and is, where weight or x is) */
     int64_t x_stride[2][3], dy_stride[2][3], y_stride[2][3];
     const float* cos;
     const float* sin;

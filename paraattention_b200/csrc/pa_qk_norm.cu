@@ -124,8 +124,10 @@ int pa_qk_norm_bwd(const pa_qk_norm_args* a, void* stream) {
     if (rc != PA_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int grid = grid_of(p);
-    const bool weights = (a->dweight[0] != nullptr && a->weight[0] != nullptr) ||
-                         (a->dweight[1] != nullptr && a->weight[1] != nullptr && a->x[1] != nullptr);
+    for (int i = 0; i < 2; ++i)
+        if (a->dweight[i] != nullptr && (a->weight[i] == nullptr || a->x[i] == nullptr))
+            return fail(PA_EINVAL, "qk_norm: dweight[%d] without x[%d] and weight[%d]", i, i, i);
+    const bool weights = a->dweight[0] != nullptr || a->dweight[1] != nullptr;
     if (weights) {
         if (a->workspace == nullptr || off16(a->workspace) ||
             a->workspace_bytes < static_cast<int64_t>(grid) * 2 * a->head_dim * static_cast<int64_t>(sizeof(float)))
@@ -134,9 +136,7 @@ int pa_qk_norm_bwd(const pa_qk_norm_args* a, void* stream) {
     }
     rc = run<true>(a, p, grid, s);
     if (rc != PA_OK || !weights) return rc;
-    uint16_t* dw[2];
-    for (int i = 0; i < 2; ++i)
-        dw[i] = (a->weight[i] != nullptr && a->x[i] != nullptr) ? static_cast<uint16_t*>(a->dweight[i]) : nullptr;
+    uint16_t* dw[2] = {static_cast<uint16_t*>(a->dweight[0]), static_cast<uint16_t*>(a->dweight[1])};
     const dim3 block(32, 32), blocks(2 * a->head_dim / 32);
     if (a->dtype == PA_BF16) pa::qk_norm_dw_kernel<true><<<blocks, block, 0, s>>>(p.dw_part, grid, a->head_dim, dw[0], dw[1]);
     else pa::qk_norm_dw_kernel<false><<<blocks, block, 0, s>>>(p.dw_part, grid, a->head_dim, dw[0], dw[1]);
