@@ -69,14 +69,12 @@ int run(const pa_xattn_args* a, const BwdPlan& f, cudaStream_t s) {
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     pa::XBwdParams p;
     memset(&p, 0, sizeof(p));
-    p.batch = a->batch;
     p.kv_batch = a->kv_batch;
     p.hkv = a->kv_heads;
     p.group = a->heads / a->kv_heads;
     p.sq = a->seq_q;
     p.skv = a->seq_kv;
     p.mt = f.mt;
-    p.kt = f.kt;
     p.scale = a->scale;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.by_group = pa::x_div(p.group);

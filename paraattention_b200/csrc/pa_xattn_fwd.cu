@@ -114,7 +114,6 @@ int run_tiles(const pa_xattn_args* a, const FwdPlan& f, cudaStream_t s) {
     if (rc != PA_OK) return rc;
     pa::XFwdParams p;
     memset(&p, 0, sizeof(p));
-    p.batch = a->batch;
     p.kv_batch = a->kv_batch;
     p.hkv = a->kv_heads;
     p.group = a->heads / a->kv_heads;

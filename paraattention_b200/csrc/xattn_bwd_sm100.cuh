@@ -62,8 +62,8 @@ constexpr int kXShiftP = 14;
 constexpr int kXBoundParts = 32;
 
 struct XBwdParams {
-    int batch, kv_batch, hkv, group, sq, skv;
-    int mt, kt;       // 128-row tiles of the queries / of the keys
+    int kv_batch, hkv, group, sq, skv;
+    int mt;           // 128-row tiles of the queries
     float scale, scale_log2;
     uint16_t* g[2];   // query pass: dq, -; key pass: dk, dv (written with TMA, but for joined or empty tiles)
     long long g_sb[2], g_sh[2], g_ss[2];

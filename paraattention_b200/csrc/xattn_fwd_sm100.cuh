@@ -36,7 +36,7 @@ constexpr int kXFwdMmaWarp = 16, kXFwdTmaWarp = 17, kXFwdCleanWarp = 18;
 constexpr int kXFwdThreads = 640;
 
 struct XFwdParams {
-    int batch, kv_batch, hkv, group, sq, skv, mt;
+    int kv_batch, hkv, group, sq, skv, mt;
     float scale, scale_log2;
     uint16_t* out;  // (the joining kernel's; the main kernel stores through its tensor map)
     long long o_sb, o_sh, o_ss;
