@@ -241,8 +241,9 @@ int pa_qkv_prep(const pa_qkv_prep_args* args, void* stream);
  *
  * pa_xattn_fwd writes out and, if non-NULL, lse [batch, heads, seq_q] (fp32, natural log).
  * pa_xattn_bwd reads q, k, v, out, lse (of the forward call) and dout and writes dq, dk, dv whole
- * (dq may be NULL, or dk and dv: not wanted, and not computed); with kv_batch = 1 dk and dv are the sums over the batch. Sums are fp32 in a fixed order: equal
- * calls on equal devices give equal bits.
+ * (dq may be NULL, or dk and dv: not wanted, and not computed); with kv_batch = 1 dk and dv are the
+ * sums over the batch. Sums are fp32 in a fixed order: equal calls on equal devices give equal bits. In
+ * PA_F16 dout may have any size that the results can be held in: what lies between is scaled.
  *
  * workspace: pa_xattn_workspace_bytes(args, backward) bytes (0 possible; depends on the current
  * device's SM count), 256-byte aligned; calls that may overlap must not share it. status and

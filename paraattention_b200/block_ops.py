@@ -5,10 +5,10 @@ rotation (``qk_norm_rotary``). Both are re-exported by :mod:`paraattention_b200.
 Like the other ops of this package they are CUDA-only, launch on the current stream, never
 synchronise, and raise instead of falling back. Both carry gradients: outside ``torch.no_grad()``,
 with an input that requires a gradient, the call is recorded and its backward pass is a kernel of
-libpa_b200 too (first derivatives in reverse mode only; a tensor with a forward-mode tangent is refused). The arguments are checked here; the rest of a call -
-output and scratch memory from PyTorch's caching allocator (so concurrent streams and captured
-graphs never share scratch), the C ABI's argument structures, the autograd node - is the extension
-_pa_torch.so (csrc/pa_torch.cpp).
+libpa_b200 too (first derivatives in reverse mode only; a tensor with a forward-mode tangent is
+refused). The arguments are checked here; the rest of a call - output and scratch memory from
+PyTorch's caching allocator (so concurrent streams and captured graphs never share scratch), the C
+ABI's argument structures, the autograd node - is the extension _pa_torch.so (csrc/pa_torch.cpp).
 """
 from __future__ import annotations
 
@@ -78,7 +78,9 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     of another length: ``softmax(scale * query key^T) value``.
 
     ``Hq`` is a multiple of ``Hkv`` (shared key heads: query head h reads key head h // (Hq // Hkv));
-    key and value may have batch size 1, one set of states for the whole batch. D is 64 or 128, bf16
+    key and value may have batch size 1, one set of states for the whole batch: with gradients, that is the form to
+    give them in. (States expanded to the batch are copied once per batch entry then, in the forward and in the
+    backward pass, and PyTorch adds up the entries' gradients in 16 bits.) D is 64 or 128, bf16
     or f16, any strides. ``key_mask``: boolean, True = the key takes part, [B, Skv] or [1, Skv] (or an
     attention mask broadcastable to [B, 1, 1, Skv]); what masked keys and values hold does not matter.
     A query without any key gets zeros (and an LSE of -inf, and no gradient). ``scale`` defaults to
